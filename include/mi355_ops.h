@@ -5,7 +5,7 @@
  * buffers (e.g. torch tensors) so that each fused stage can be checked against the oracle at
  * its own scale and timed on its own (bench.py roofline leg).  They are not needed to use the
  * engine.  Every call runs on the HIP null stream of the current device and synchronises
- * before returning.  Error convention as in mi355_decode.h.
+ * before returning (mi_op_bounded_* only enqueue, on the caller's stream).  Error convention as in mi355_decode.h.
  *
  * Reference op each one replaces (MLX call sites in the reference):
  *   mi_op_gemv        nn.Linear / nn.QuantizedLinear (+ fused RMSNorm / residual / SwiGLU):
@@ -153,6 +153,60 @@ int mi_op_gemm_prefill_pays(int codes, int hilo, int rounded, int rows);
 int mi_op_sample(float* logits, int B, int V, float temperature, float top_p, const float* uniforms,
                  int top_logprobs, int32_t* tokens_out, float* logprob_out, float* prob_row0_out,
                  int32_t* topk_ids, float* topk_logprobs, float* row_stats);
+
+/* ---- a cache of fixed size -------------------------------------------------------------------------------------------------------
+ * Keys and values of `rows` sequences in at most `cap` slots each: when a row grows past a budget, the keys that attention has looked at
+ * least leave.  The slot of a key and its position in the sequence are two things: keys are cached rotated, softmax does not ask for their
+ * order, and after an eviction slots are in no order of position.
+ *
+ * These calls enqueue on `stream` (a hipStream_t of the current device, NULL: its null stream) and return; they may be captured into a graph.
+ * Calls on one cache follow one another in the order of its stream; ws is the call's own until it has run.  All pointers are device memory,
+ * arrays are contiguous and aligned to 16 bytes.  What lies in `len`, `next`, `counts` and the block table is read on the device and cannot be refused: a
+ * length outside [0, cap] counts as the nearer end, a table entry outside [0, n_blocks) names no block: its keys take no part in attention, and nothing is
+ * written for them.  Slots behind a row's length keep what they hold. */
+typedef struct mi_op_bounded_cache {
+  int32_t rows, Hkv, D, dtype;       /* D: 16, 32, 64, 96, 128, 192, 256; dtype MI_F32 / MI_BF16 / MI_F16: of K, V, queries, outputs and norm weights */
+  int32_t cap;                       /* slots per row (paged: at most bt_stride blocks) */
+  int32_t n_blocks, bt_stride, bs_shift;   /* paged: blocks in the arena, table entries per row, blocks of 1 << bs_shift >= 16 tokens */
+  void* k; void* v;                  /* [rows][Hkv][cap][D]; paged: [n_blocks][Hkv][1 << bs_shift][D], a block belongs to one row */
+  const int32_t* btab;               /* [rows][bt_stride], or NULL: not paged */
+  int32_t* len; int32_t* next;       /* [rows] slots filled; position of the row's next token */
+  int32_t* pos; float* weight;       /* [rows][Hkv][cap] position of the key in a slot; attention weight that it has received */
+} mi_op_bounded_cache;
+
+/* New tokens: queries and keys are normed per head (x / sqrt(mean x^2 + eps) * w; no norm where the weights are NULL), rotated by the angles of their
+ * positions (pairs i, i + D / 2), keys and values go to the slots from len on, with their positions and weight 0; len and next move on.
+ * A row takes min(counts, L, cap - len, max_pos - next) tokens (counts NULL: L), its first ones; queries of the others are zeros. */
+typedef struct mi_op_bounded_tokens {
+  const void* qkv;                   /* token t of row r: [(Hq + 2 Hkv) * D] at r * ld_row + t * ld_token elements (strides: whole 16 bytes) */
+  int64_t ld_row, ld_token;
+  int32_t L, Hq;
+  const int32_t* counts;             /* [rows] or NULL */
+  const void* q_norm_w; const void* k_norm_w;      /* [D] each or NULL */
+  float eps;
+  int32_t max_pos;
+  const float* cos_tab; const float* sin_tab;      /* [max_pos][D / 2] (mi_op_rope_tables) */
+  void* q_out;                       /* [rows][L][Hq][D] */
+} mi_op_bounded_tokens;
+int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_tokens* t, void* stream);
+
+/* Attention of one query per row and head, q and out [rows][Hq][D], over all keys that the row holds (its own, just appended, among them); the weight that
+ * every key receives, summed over the query heads of its KV head, is added to `weight`.  A row with nothing to see, or with counts[row] <= 0, gives zeros.
+ * Hq / Hkv <= 128, scale > 0.  ws_bytes: mi_op_bounded_attend_ws, which needs no pointer. */
+uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq);
+int mi_op_bounded_attend(const mi_op_bounded_cache* c, const void* q, int Hq, const int32_t* counts, float scale, void* out, void* ws, uint64_t ws_bytes, void* stream);
+
+/* The same weights (no output) for the queries of a prompt: q [rows][L][Hq][D], of which row r has counts[r] (NULL: L); they belong to its last counts[r]
+ * slots, and each sees those up to its own.  last > 0: only the last `last` of them ask. */
+uint64_t mi_op_bounded_weigh_ws(const mi_op_bounded_cache* c, int L, int Hq, int last);
+int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int Hq, const int32_t* counts, int last, float scale, void* ws, uint64_t ws_bytes,
+                        void* stream);
+
+/* At most `budget` keys stay in every row: for each KV head first those at positions below keep_first or among the keep_last before `next`, then by
+ * weight (NaN: as -inf), equal ones by the lower slot.  What stays behind slot `budget` moves into the holes in front of it, the i-th into the
+ * i-th, with its position and weight; len becomes min(len, budget).  keep_first + keep_last <= budget. */
+uint64_t mi_op_bounded_evict_ws(const mi_op_bounded_cache* c, int budget);
+int mi_op_bounded_evict(const mi_op_bounded_cache* c, int budget, int keep_first, int keep_last, void* ws, uint64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -96,6 +96,18 @@ class OpAttnShape(C.Structure):
                 ("act", C.c_int32), ("kv", C.c_int32), ("rnd", C.c_int32), ("cap", C.c_int32)]
 
 
+class OpBoundedCache(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32), ("cap", C.c_int32),
+                ("n_blocks", C.c_int32), ("bt_stride", C.c_int32), ("bs_shift", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("btab", C.c_void_p), ("len", C.c_void_p), ("next", C.c_void_p), ("pos", C.c_void_p), ("weight", C.c_void_p)]
+
+
+class OpBoundedTokens(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("ld_row", C.c_int64), ("ld_token", C.c_int64), ("L", C.c_int32), ("Hq", C.c_int32), ("counts", C.c_void_p),
+                ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("eps", C.c_float), ("max_pos", C.c_int32), ("cos_tab", C.c_void_p),
+                ("sin_tab", C.c_void_p), ("q_out", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol the two headers declare
 _P = C.c_void_p
 _I32P = C.POINTER(C.c_int32)
@@ -164,6 +176,13 @@ SIGNATURES = {
     "mi_op_gemm_q4_prepared": (C.c_int, [C.POINTER(OpLinear), C.POINTER(OpGemvArgs)]),
     "mi_op_attention_mixed": (C.c_int, [C.POINTER(OpAttnShape), C.POINTER(OpAttnShape), C.c_int, C.c_int]),
     "mi_op_gemm_prefill_pays": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "mi_op_bounded_append": (C.c_int, [C.POINTER(OpBoundedCache), C.POINTER(OpBoundedTokens), _P]),
+    "mi_op_bounded_attend_ws": (C.c_uint64, [C.POINTER(OpBoundedCache), C.c_int]),
+    "mi_op_bounded_attend": (C.c_int, [C.POINTER(OpBoundedCache), _P, C.c_int, _P, C.c_float, _P, _P, C.c_uint64, _P]),
+    "mi_op_bounded_weigh_ws": (C.c_uint64, [C.POINTER(OpBoundedCache), C.c_int, C.c_int, C.c_int]),
+    "mi_op_bounded_weigh": (C.c_int, [C.POINTER(OpBoundedCache), _P, C.c_int, C.c_int, _P, C.c_int, C.c_float, _P, C.c_uint64, _P]),
+    "mi_op_bounded_evict_ws": (C.c_uint64, [C.POINTER(OpBoundedCache), C.c_int]),
+    "mi_op_bounded_evict": (C.c_int, [C.POINTER(OpBoundedCache), C.c_int, C.c_int, C.c_int, _P, C.c_uint64, _P]),
     "mi_op_sample": (C.c_int, [_P, C.c_int, C.c_int, C.c_float, C.c_float, _P, C.c_int, _P, _P, _P, _P, _P, _P]),
 }
 

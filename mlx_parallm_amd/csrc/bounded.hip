@@ -1,0 +1,937 @@
+// bounded.hip -- a cache of fixed size (mi_op_bounded_*, include/mi355_ops.h): append, attention of one new token that also says what weight
+// every key received, the same weights for the queries of a prompt, eviction of the least weighted keys.
+//
+// The slot that a key lies in and its position in the sequence are two things here: after an eviction they differ.  Softmax does not ask for
+// the order of keys (they are cached rotated), so a cache may hold them in any order, and an eviction moves the kept keys behind the new end
+// into the holes in front of it and nothing else.
+#include <algorithm>
+
+#include "attn_prefill_body.h"
+
+namespace mi {
+
+namespace {
+
+using prefill::f32x4;
+using prefill::mfma16;
+using prefill::pack2_split;
+using prefill::u32x2;
+using prefill::u32x4;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SPLITS = 64;          // slices of a row's keys
+constexpr int MAX_GROUP = 128;          // query heads per KV head
+
+__device__ __forceinline__ int held_keys(const BoundedCache& c, int r) { return min(max(c.len[r], 0), c.cap); }
+
+// Places of 16 keys that begin at a multiple of 16: one block of a paged cache (blocks are powers of two from 16 on).  The index of the first
+// key's row of D elements; -1 where the table names no block of the arena (its keys take no part).
+__device__ __forceinline__ int64_t row_of_16(const BoundedCache& c, int r, int h, int key) {
+  if (c.btab == nullptr) return ((int64_t)r * c.Hkv + h) * c.cap + key;
+  const int blk = c.btab[(size_t)r * c.bt_stride + (key >> c.bs_shift)];
+  if ((unsigned)blk >= (unsigned)c.n_blocks) return -1;
+  return (((int64_t)blk * c.Hkv + h) << c.bs_shift) + (key & ((1 << c.bs_shift) - 1));
+}
+
+// raw bits of NB bytes (2, or a multiple of 4)
+template <int NB>
+struct Raw { uint32_t w[(NB + 3) / 4]; };
+template <int NB>
+__device__ __forceinline__ Raw<NB> load_bits(const void* p) {
+  Raw<NB> o;
+  if constexpr (NB % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 16; ++i) {
+      const u32x4 v = ((const u32x4*)p)[i];
+      o.w[4 * i] = v.x; o.w[4 * i + 1] = v.y; o.w[4 * i + 2] = v.z; o.w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (NB % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 8; ++i) {
+      const u32x2 v = ((const u32x2*)p)[i];
+      o.w[2 * i] = v.x; o.w[2 * i + 1] = v.y;
+    }
+  } else if constexpr (NB % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < NB / 4; ++i) o.w[i] = ((const uint32_t*)p)[i];
+  } else {
+    o.w[0] = *(const uint16_t*)p;
+  }
+  return o;
+}
+
+// ---- append ---------------------------------------------------------------------------------------------------------------------------
+// One lane takes 8 + 8 elements of a head, i .. i + 8 and i + D / 2 .. i + D / 2 + 8 (the two halves of a rotation's pairs), a power of two of
+// lanes a head.  All in 32 bits, rounded once, to what is stored.
+// STEP (one token a row): a workgroup per row, which moves the row's length and next position itself.  Otherwise the tasks of all tokens lie
+// side by side and a second launch moves them.
+template <typename T>
+struct alignas(16) Vec8 { T v[8]; };
+
+template <typename T, bool STEP>
+__global__ __launch_bounds__(STEP ? 1024 : 256) void append_kernel(BoundedCache c, BoundedTokens t, int lane_bits) {
+  const int nh = t.Hq + 2 * c.Hkv, D = c.D, D2 = D / 2, lanes = 1 << lane_bits;
+  const int per_token = nh << lane_bits;
+  const int64_t total = STEP ? per_token : (int64_t)c.rows * t.L * per_token;
+  int n_step = 0, len_step = 0, next_step = 0;
+  for (int64_t task = STEP ? threadIdx.x : (int64_t)blockIdx.x * 256 + threadIdx.x; task < total; task += STEP ? 1024 : total) {
+    const int64_t token = STEP ? blockIdx.x : task / per_token;
+    const int in_token = (int)(STEP ? task : task - token * per_token);
+    const int r = (int)(token / t.L), i = (int)(token - (int64_t)r * t.L);
+    const int head = in_token >> lane_bits, e0 = (in_token & (lanes - 1)) * 8;
+    const int len = held_keys(c, r), next = c.next[r];
+    const int n = t.count(c, r, len, next);
+    const bool is_q = head < t.Hq, is_k = !is_q && head < t.Hq + c.Hkv;
+    const bool has = e0 < D2;                    // (lanes beyond the head's size: D = 96, 192)
+    Vec8<T> a{}, b{};
+    T* dst = nullptr;
+    if (i < n) {
+      const T* src = (const T*)t.qkv + (int64_t)r * t.ld_row + (int64_t)i * t.ld_token + (int64_t)head * D + e0;
+      if (has) { a = *(const Vec8<T>*)src; b = *(const Vec8<T>*)(src + D2); }
+      if (is_q || is_k) {
+        float x[8], y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { x[j] = (float)a.v[j]; y[j] = (float)b.v[j]; }
+        const T* nw = (const T*)(is_q ? t.q_norm_w : t.k_norm_w);
+        if (nw != nullptr) {
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], fmaf(y[j], y[j], ss));
+          for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor(ss, o, 64);
+          const float rs = 1.0f / sqrtf(ss / (float)D + t.eps);
+          if (has) {
+            const Vec8<T> wa = *(const Vec8<T>*)(nw + e0), wb = *(const Vec8<T>*)(nw + e0 + D2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { x[j] *= rs * (float)wa.v[j]; y[j] *= rs * (float)wb.v[j]; }
+          }
+        }
+        if (has) {
+          const float* cp = t.cos_tab + (int64_t)(next + i) * D2 + e0;
+          const float* sp = t.sin_tab + (int64_t)(next + i) * D2 + e0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            a.v[j] = (T)(x[j] * cp[j] - y[j] * sp[j]);
+            b.v[j] = (T)(y[j] * cp[j] + x[j] * sp[j]);
+          }
+        }
+      }
+      if (!is_q) {
+        const int kh = is_k ? head - t.Hq : head - t.Hq - c.Hkv, slot = len + i;
+        const int64_t at = row_of_16(c, r, kh, slot & ~15);
+        if (at >= 0) dst = (T*)(is_k ? c.k : c.v) + (at + (slot & 15)) * D + e0;
+        if (is_k && e0 == 0) {
+          const size_t m = ((size_t)r * c.Hkv + kh) * c.cap + slot;
+          c.pos[m] = next + i;
+          c.weight[m] = 0.f;
+        }
+      }
+    }
+    if (is_q) dst = (T*)t.q_out + (token * t.Hq + head) * D + e0;       // (zeros for tokens that are not taken)
+    if (dst != nullptr && has) { *(Vec8<T>*)dst = a; *(Vec8<T>*)(dst + D2) = b; }
+    n_step = n; len_step = len; next_step = next;
+  }
+  if constexpr (STEP) {
+    __syncthreads();                             // every thread has read them
+    if (threadIdx.x == 0) { c.len[blockIdx.x] = len_step + n_step; c.next[blockIdx.x] = next_step + n_step; }
+  }
+}
+
+__global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
+  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= c.rows) return;
+  const int len = held_keys(c, r), next = c.next[r], n = t.count(c, r, len, next);
+  c.len[r] = len + n;
+  c.next[r] = next + n;
+}
+
+// ---- attend ---------------------------------------------------------------------------------------------------------------------------
+// Everything is laid out so that nothing crosses lanes: S^T = K Q^T leaves in a lane the scores of one query head (its column, lane & 15) and of
+// the keys that the same lane multiplies in O^T += V^T P^T, and every rescale is the lane's own.  16-bit: a tile is 32 keys, 16 x 16 x 32
+// products; the slot k = 8 q + 4 t + i of the second product stands for key 16 t + 4 q + i (q = lane >> 4), which is where the first left
+// it.  A lane loads E = D / 16 elements of 8 keys' values -- whole rows across 16 lanes -- and transposes its 8 x E block in registers
+// (v_perm); column n of output tile j is element n E + j.  P goes in as two 16-bit terms (2^-17).  float32: 16 x 16 x 4 products, no
+// transposition.  The largest score so far is taken in when a new one exceeds it by 2^8, not at every tile.
+// A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
+template <typename T, int D>
+struct Frag {
+  static constexpr int PE = 16 / (int)sizeof(T), N = (D + 4 * PE - 1) / (4 * PE);
+  u32x4 w[N];
+  __device__ __forceinline__ void load(const T* row, int qd, bool ok = true) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int e = (4 * c + qd) * PE;
+      if (D % (4 * PE) != 0) ok = ok && e < D;
+      w[c] = ok ? *(const u32x4*)(row + e) : u32x4{0, 0, 0, 0};
+    }
+  }
+};
+template <typename T, int D>
+__device__ __forceinline__ f32x4 dot16(const Frag<T, D>& a, const Frag<T, D>& b) {          // 16 rows of a by 16 rows of b
+  f32x4 s{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < Frag<T, D>::N; ++c) {
+    if constexpr (sizeof(T) == 2) {
+      s = mfma16<T>(a.w[c], b.w[c], s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.w[c][e]), __uint_as_float(b.w[c][e]), s, 0, 0, 0);
+    }
+  }
+  return s;
+}
+
+template <int E>
+__device__ __forceinline__ u32x4 column(const Raw<E * 2> (&v)[8], int j) {         // element j of 8 rows
+  uint32_t o[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    if constexpr (E == 1) o[p] = v[2 * p].w[0] | (v[2 * p + 1].w[0] << 16);
+    else o[p] = __builtin_amdgcn_perm(v[2 * p + 1].w[j / 2], v[2 * p].w[j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+  }
+  return u32x4{o[0], o[1], o[2], o[3]};
+}
+
+// O^T += V^T P^T for the keys of a tile: v[4 t + i] is this lane's E elements of key 16 t + 4 q + i, p[t][i] that key's weight
+template <typename T, int E>
+__device__ __forceinline__ void add_values(const Raw<E * 2> (&v)[8], const float (&p)[2][4], f32x4 (&o)[E]) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    pack2_split<T>(p[t][0], p[t][1], hi[2 * t], lo[2 * t]);
+    pack2_split<T>(p[t][2], p[t][3], hi[2 * t + 1], lo[2 * t + 1]);
+  }
+  const u32x4 ph{hi[0], hi[1], hi[2], hi[3]}, pl{lo[0], lo[1], lo[2], lo[3]};
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const u32x4 a = column<E>(v, j);
+    o[j] = mfma16<T>(a, ph, o[j]);
+    o[j] = mfma16<T>(a, pl, o[j]);
+  }
+}
+template <typename T, int E, int SUB>
+__device__ __forceinline__ void add_values(const Raw<E * 4> (&v)[4 * SUB], const float (&p)[SUB][4], f32x4 (&o)[E]) {
+#pragma unroll
+  for (int t = 0; t < SUB; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[4 * t + i].w[j]), p[t][i], o[j], 0, 0, 0);
+}
+
+// the slice of a row's keys that each of `splits` workgroups takes: a multiple of 128 (one tile of 32 for each of four waves)
+__device__ __forceinline__ int slice_keys(int n, int splits) { return ((n + splits - 1) / splits + 127) & ~127; }
+
+// Workspace of a call: scores [row][KV head][query head of the group][cap, in 32s] as products (no scale), then of every slice the largest score
+// and the sum [row][KV head][slice][head][2], then its output [row][KV head][slice][head][D].
+struct AttendWs {
+  float* scores; float* stats; float* part; int ld;
+};
+
+template <typename T, int E>
+__global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
+  constexpr int D = 16 * E, NW = 4;
+  constexpr int SUB = sizeof(T) == 4 && E > 8 ? 1 : 2, KT = 16 * SUB;      // (float32 heads of 192 and 256: registers for 16 keys)
+  const int G = a.Hq / c.Hkv, split = blockIdx.x, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv, h0 = blockIdx.z * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
+  const int heads = min(16, G - h0);
+  const bool alone = splits == 1 && gridDim.z == 1;     // nothing to join: this workgroup writes the results
+  const bool idle = a.counts != nullptr && a.counts[r] <= 0;
+  const int n = idle ? 0 : held_keys(c, r);
+  const int chunk = slice_keys(n, splits), s0 = split * chunk, s1 = min(n, s0 + chunk);
+  T* out = (T*)a.out + ((size_t)r * a.Hq + kh * G + h0) * D;
+  if (s0 >= s1 && !(alone && split == 0)) return;       // (the joining launch knows which slices there are)
+
+  __shared__ float sh_m[NW][16], sh_l[NW][16];
+  __shared__ float sh_o[NW][16][D + 4];                 // (+ 4: the four quarters of a wave on different banks)
+
+  Frag<T, D> q, k[SUB];
+  Raw<E * (int)sizeof(T)> v[4 * SUB];
+  q.load((const T*)a.q + ((size_t)r * a.Hq + kh * G + h0 + ln) * D, qd, ln < heads);
+  const float sc = a.scale * LOG2E;
+  float m = -1e30f, l = 0.f;
+  f32x4 o[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;
+
+  for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
+    bool there[SUB];
+#pragma unroll
+    for (int t = 0; t < SUB; ++t) {
+      const int key = __builtin_amdgcn_readfirstlane(base + 16 * t);
+      const int64_t at = key < s1 ? row_of_16(c, r, kh, key) : -1;
+      there[t] = at >= 0;
+      const int last = there[t] ? min(15, s1 - 1 - key) : 0;           // (a clamped address: its scores are masked, its values cleared)
+      const T* kp = (const T*)c.k + (there[t] ? at : 0) * D;
+      const T* vp = (const T*)c.v + (there[t] ? at : 0) * D;
+      k[t].load(kp + (int64_t)min(ln, last) * D, qd);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * t + i] = load_bits<E * (int)sizeof(T)>(vp + (int64_t)min(4 * qd + i, last) * D + ln * E);
+    }
+    float p[SUB][4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < SUB; ++t) {
+      f32x4 s = dot16(k[t], q);
+      const int key = base + 16 * t + 4 * qd;
+      if (base + KT > s1 || !there[t]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (key + i >= s1 || !there[t]) {
+            s[i] = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
+          }
+      }
+      if (ln < heads && key < s1) *(f32x4*)(sc_out + key) = s;         // (`ld` reaches to the tile's end)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i] * sc); }
+    }
+    if (__any(top > m + 8.f)) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - now);
+      m = now; l *= f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) o[j] *= f;
+    }
+#pragma unroll
+    for (int t = 0; t < SUB; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { p[t][i] = __builtin_amdgcn_exp2f(fmaf(p[t][i], sc, -m)); l += p[t][i]; }
+    if constexpr (sizeof(T) == 2) add_values<T, E>(v, p, o);
+    else add_values<T, E, SUB>(v, p, o);
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (lane < 16) { sh_m[wave][ln] = m; sh_l[wave][ln] = l; }
+  if (ln < heads) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < E; ++j) sh_o[wave][ln][(4 * qd + i) * E + j] = o[j][i];
+  }
+  __syncthreads();
+  // the four waves' states
+  auto join = [&](int h, float& M, float& L, float (&f)[NW]) {
+    M = fmaxf(fmaxf(sh_m[0][h], sh_m[1][h]), fmaxf(sh_m[2][h], sh_m[3][h]));
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { f[w] = __builtin_amdgcn_exp2f(sh_m[w][h] - M); L = fmaf(sh_l[w][h], f[w], L); }
+  };
+  const size_t slice = ((size_t)(r * c.Hkv + kh) * splits + split) * G + h0;
+  for (int e = threadIdx.x; e < heads * D; e += 256) {
+    const int h = e / D, d = e % D;
+    float M, L, f[NW], x = 0.f;
+    join(h, M, L, f);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) x = fmaf(sh_o[w][h][d], f[w], x);
+    if (alone) {
+      out[e] = (T)(L != 0.f ? x / L : 0.f);
+    } else {
+      ws.part[slice * D + e] = x;
+      if (d == 0) { ws.stats[(slice + h) * 2] = M; ws.stats[(slice + h) * 2 + 1] = L; }
+    }
+  }
+  if (!alone || n == 0) return;
+  // what every key received: its scores lie in the workspace, written by this workgroup in front of the barrier above
+  __syncthreads();
+  if (threadIdx.x < heads) {
+    float M, L, f[NW];
+    join(threadIdx.x, M, L, f);
+    sh_o[0][0][threadIdx.x] = M;
+    sh_o[0][1][threadIdx.x] = L != 0.f ? 1.f / L : 0.f;
+  }
+  __syncthreads();
+  const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld;
+  float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
+  for (int key = threadIdx.x; key < n; key += 256) {
+    float x = 0.f;
+    for (int h = 0; h < heads; ++h) x = fmaf(__builtin_amdgcn_exp2f(fmaf(sp[(size_t)h * ws.ld + key], sc, -sh_o[0][0][h])), sh_o[0][1][h], x);
+    wp[key] += x;
+  }
+}
+
+// The slices' results joined: the output, and the weights of JOIN_KEYS keys a workgroup.
+constexpr int JOIN_KEYS = 1024;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
+  const int G = a.Hq / c.Hkv, D = c.D, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
+  const bool idle = a.counts != nullptr && a.counts[r] <= 0;
+  const int n = idle ? 0 : held_keys(c, r);
+  if (blockIdx.x > 0 && (int)blockIdx.x * JOIN_KEYS >= n) return;
+  const int chunk = slice_keys(n, splits), ns = n > 0 ? (n + chunk - 1) / chunk : 0;
+  __shared__ float sh_m[MAX_GROUP], sh_r[MAX_GROUP];
+  const float* st = ws.stats + (size_t)(r * c.Hkv + kh) * splits * G * 2;
+  for (int h = threadIdx.x >> 6; h < G; h += 4) {       // a wave per head, a lane per slice
+    const int i = threadIdx.x & 63;
+    const float m = i < ns ? st[((size_t)i * G + h) * 2] : -1e30f, M = wave_max(m);
+    const float L = wave_sum(i < ns ? st[((size_t)i * G + h) * 2 + 1] * __builtin_amdgcn_exp2f(m - M) : 0.f);
+    if (i == 0) { sh_m[h] = M; sh_r[h] = L != 0.f ? 1.f / L : 0.f; }
+  }
+  __syncthreads();
+  // the output: its elements spread over the row's workgroups
+  const int groups = max(1, (n + JOIN_KEYS - 1) / JOIN_KEYS);
+  const float* pp = ws.part + (size_t)(r * c.Hkv + kh) * splits * G * D;
+  for (int e = blockIdx.x * 256 + threadIdx.x; e < G * D; e += groups * 256) {
+    const int h = e / D;
+    float x = 0.f;
+    for (int i = 0; i < ns; ++i) x = fmaf(pp[(size_t)i * G * D + e], __builtin_amdgcn_exp2f(st[((size_t)i * G + h) * 2] - sh_m[h]), x);
+    ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
+  }
+  const float sc = a.scale * LOG2E;
+  const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld;
+  float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
+  const int k0 = blockIdx.x * JOIN_KEYS;
+  for (int key = k0 + threadIdx.x; key < min(n, k0 + JOIN_KEYS); key += 256) {
+    float x = 0.f;
+    for (int h = 0; h < G; ++h) x = fmaf(__builtin_amdgcn_exp2f(fmaf(sp[(size_t)h * ws.ld + key], sc, -sh_m[h])), sh_r[h], x);
+    wp[key] += x;
+  }
+}
+
+// ---- weigh ----------------------------------------------------------------------------------------------------------------------------
+// Queries of a row and KV head lie in one line, rho = query * G + head of the group, so that 128 of them see nearly the same keys.  Two passes
+// over S^T = K Q^T: the largest score and the sum of every query (a lane keeps its own over the keys that it holds; four lanes join at the
+// end), then the sum over the queries for every key.  The first keeps queries in registers and passes keys through LDS, the second the
+// other way round.
+struct WeighWs { float* stats; float* parts; };      // [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge
+
+struct WeighRow {                                    // what the queries of a row are
+  int n, first, queries, behind;                     // keys; first query that asks, their number; query i sees keys up to behind + i
+};
+__device__ __forceinline__ WeighRow weigh_row(const BoundedCache& c, const BoundedWeigh& a, int r) {
+  WeighRow w;
+  w.n = held_keys(c, r);
+  const int cnt = a.counts != nullptr ? min(max(a.counts[r], 0), a.L) : a.L;
+  w.first = a.last > 0 ? max(0, cnt - a.last) : 0;
+  w.queries = cnt - w.first;
+  w.behind = w.n - cnt;
+  return w;
+}
+
+constexpr int STAT_QUERIES = 128;
+template <typename T, int D>
+constexpr int tile_rows() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }                  // rows of a tile in LDS: two tiles of 16 KiB
+
+// 256 threads hold a tile of ROWS rows in registers on its way from memory to LDS
+template <typename T, int D, int ROWS>
+struct Stage {
+  static constexpr int PER = D * (int)sizeof(T) / 16, LD = D * (int)sizeof(T) + 16;        // pieces a row; bytes a row in LDS (16 more: rows on different banks)
+  static constexpr int N = (ROWS * PER + 255) / 256;
+  u32x4 w[N];
+  template <typename F>
+  __device__ __forceinline__ void load(F&& row) {                                          // row(i): its address, or null for zeros
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      const int p = threadIdx.x + s * 256, i = p / PER;
+      const T* at = ROWS * PER % 256 == 0 || i < ROWS ? row(i) : nullptr;
+      w[s] = at != nullptr ? *(const u32x4*)((const char*)at + p % PER * 16) : u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      const int p = threadIdx.x + s * 256, i = p / PER;
+      if (ROWS * PER % 256 == 0 || i < ROWS) *(u32x4*)(lds + i * LD + p % PER * 16) = w[s];
+    }
+  }
+};
+
+// (float32 heads of 256: one wave a SIMD, or the queries spill)
+template <typename T, int E>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_stats_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits) {
+  constexpr int D = 16 * E, ROWS = tile_rows<T, D>();
+  using St = Stage<T, D, ROWS>;
+  const int G = a.Hq / c.Hkv, kh = blockIdx.z % c.Hkv, r = blockIdx.z / c.Hkv, split = blockIdx.y;
+  const WeighRow w = weigh_row(c, a, r);
+  const int rho0 = (gridDim.x - 1 - blockIdx.x) * STAT_QUERIES, rhos = w.queries * G;      // (the queries that see most keys first)
+  if (rho0 >= rhos) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
+  __shared__ __align__(16) char tiles[2][ROWS * St::LD];
+
+  Frag<T, D> q[2];
+  int sees[2];                                           // keys that the column's query sees
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int rho = rho0 + wave * 32 + u * 16 + ln;
+    const int i = w.first + rho / G, g = rho % G;
+    sees[u] = rho < rhos ? w.behind + i + 1 : 0;
+    q[u].load((const T*)a.q + (((size_t)r * a.L + min(i, a.L - 1)) * a.Hq + kh * G + g) * D, qd, rho < rhos);
+  }
+  // the keys of this slice that any query of the workgroup sees, and how many of them all see
+  const int most = w.behind + w.first + (min(rhos, rho0 + STAT_QUERIES) - 1) / G + 1;
+  const int all = rho0 + STAT_QUERIES <= rhos ? w.behind + w.first + rho0 / G + 1 : 0;
+  const int chunk = ((max(most, 0) + splits - 1) / splits + ROWS - 1) / ROWS * ROWS;
+  const int s0 = split * chunk, s1 = min(most, s0 + chunk);
+  const float sc = a.scale * LOG2E;
+  float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
+  St st;
+  auto fetch = [&](int base) {
+    st.load([&](int i) -> const T* {
+      const int key = base + i;
+      if (key >= s1) return nullptr;
+      const int64_t at = row_of_16(c, r, kh, key & ~15);
+      return at < 0 ? nullptr : (const T*)c.k + (at + (key & 15)) * D;
+    });
+  };
+  if (s0 < s1) { fetch(s0); st.store(tiles[0]); }
+  __syncthreads();
+  int cur = 0;
+  for (int base = s0; base < s1; base += ROWS, cur ^= 1) {
+    const bool more = base + ROWS < s1;
+    if (more) fetch(base + ROWS);
+    const char* tile = tiles[cur];
+    const bool edge = base + ROWS > min(all, s1) || c.btab != nullptr;
+#pragma unroll
+    for (int t0 = 0; t0 < ROWS / 16; t0 += 2) {
+      Frag<T, D> k[2];
+      f32x4 s[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        k[t].load((const T*)(tile + ((t0 + t) * 16 + ln) * St::LD), qd);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[t][u] = dot16(k[t], q[u]);
+      }
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int key = base + (t0 + t) * 16;
+          const bool there = c.btab == nullptr || key >= s1 || row_of_16(c, r, kh, key) >= 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (key + 4 * qd + i >= min(sees[u], s1) || !there) s[t][u][i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float top = m[u];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i] * sc);
+        float x = l[u] * __builtin_amdgcn_exp2f(m[u] - top);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x += __builtin_amdgcn_exp2f(fmaf(s[t][u][i], sc, -top));
+        m[u] = top; l[u] = x;
+      }
+    }
+    if (more) st.store(tiles[cur ^ 1]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1) {
+      const float mo = __shfl_xor(m[u], off, 64), lo = __shfl_xor(l[u], off, 64), M = fmaxf(m[u], mo);
+      l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - M) + lo * __builtin_amdgcn_exp2f(mo - M);
+      m[u] = M;
+    }
+    const int rho = rho0 + wave * 32 + u * 16 + ln;
+    if (qd == 0 && rho < rhos) {
+      const size_t R = (size_t)a.L * G, rk = (size_t)r * c.Hkv + kh;
+      if (splits == 1) {
+        ws.stats[(rk * R + rho) * 2] = l[u] != 0.f ? m[u] : 0.f;
+        ws.stats[(rk * R + rho) * 2 + 1] = l[u] != 0.f ? 1.f / l[u] : 0.f;
+      } else {
+        float* o = ws.parts + ((rk * splits + split) * R + rho) * 2;
+        o[0] = m[u]; o[1] = l[u];
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits) {
+  const int G = a.Hq / c.Hkv, r = blockIdx.y / c.Hkv;
+  const WeighRow w = weigh_row(c, a, r);
+  const int rho = blockIdx.x * 256 + threadIdx.x;
+  if (rho >= w.queries * G) return;
+  const size_t R = (size_t)a.L * G, rk = blockIdx.y;
+  float M = -1e30f, L = 0.f;
+  for (int i = 0; i < splits; ++i) M = fmaxf(M, ws.parts[((rk * splits + i) * R + rho) * 2]);
+  for (int i = 0; i < splits; ++i) {
+    const float* p = ws.parts + ((rk * splits + i) * R + rho) * 2;
+    L = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - M), L);
+  }
+  ws.stats[(rk * R + rho) * 2] = L != 0.f ? M : 0.f;
+  ws.stats[(rk * R + rho) * 2 + 1] = L != 0.f ? 1.f / L : 0.f;
+}
+
+template <typename T, int E, int KS>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_add_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws) {
+  constexpr int D = 16 * E, ROWS = tile_rows<T, D>();
+  using St = Stage<T, D, ROWS>;
+  const int G = a.Hq / c.Hkv, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
+  const WeighRow w = weigh_row(c, a, r);
+  const int j0 = blockIdx.x * 64 * KS;
+  if (j0 >= w.n || w.queries <= 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
+  __shared__ __align__(16) char tiles[2][ROWS * St::LD];
+  __shared__ float2 stats[2][ROWS];
+
+  const int my0 = j0 + wave * 16 * KS;
+  Frag<T, D> k[KS];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) {
+    const int key = my0 + 16 * t;
+    const int64_t at = key < w.n ? row_of_16(c, r, kh, key) : -1;
+    k[t].load((const T*)c.k + ((at < 0 ? 0 : at) + min(ln, max(0, w.n - 1 - key))) * D, qd, at >= 0);
+  }
+  const int rhos = w.queries * G;
+  const int from = max(0, j0 - w.behind - w.first) * G;            // the first query that sees key j0
+  const float sc = a.scale * LOG2E;
+  const size_t R = (size_t)a.L * G, rk = (size_t)r * c.Hkv + kh;
+  float x[KS][4];
+#pragma unroll
+  for (int t = 0; t < KS; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[t][i] = 0.f;
+  St st;
+  float2 sv = make_float2(0.f, 0.f);
+  auto fetch = [&](int base) {
+    st.load([&](int i) -> const T* {
+      const int rho = base + i;
+      return rho < rhos ? (const T*)a.q + (((size_t)r * a.L + w.first + rho / G) * a.Hq + kh * G + rho % G) * D : nullptr;
+    });
+    if (threadIdx.x < ROWS) sv = base + (int)threadIdx.x < rhos ? *(const float2*)(ws.stats + (rk * R + base + threadIdx.x) * 2) : make_float2(0.f, 0.f);
+  };
+  if (from < rhos) {
+    fetch(from);
+    st.store(tiles[0]);
+    if (threadIdx.x < ROWS) stats[0][threadIdx.x] = sv;
+  }
+  __syncthreads();
+  int cur = 0;
+  for (int base = from; base < rhos; base += ROWS, cur ^= 1) {
+    const bool more = base + ROWS < rhos;
+    if (more) fetch(base + ROWS);
+    const char* tile = tiles[cur];
+    const bool edge = w.behind + w.first + base / G + 1 < my0 + 16 * KS;      // the tile's first query does not see all keys of this wave
+#pragma unroll
+    for (int u = 0; u < ROWS / 16; ++u) {
+      Frag<T, D> q;
+      q.load((const T*)(tile + (u * 16 + ln) * St::LD), qd);
+      const float2 ml = stats[cur][u * 16 + ln];
+      const int sees = w.behind + w.first + (base + u * 16 + ln) / G + 1;
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const f32x4 s = dot16(k[t], q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -ml.x));
+          if (edge && my0 + 16 * t + 4 * qd + i >= sees) p = 0.f;
+          x[t][i] = fmaf(p, ml.y, x[t][i]);
+        }
+      }
+    }
+    if (more) {
+      st.store(tiles[cur ^ 1]);
+      if (threadIdx.x < ROWS) stats[cur ^ 1][threadIdx.x] = sv;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < KS; ++t) {
+    const int key0 = my0 + 16 * t;
+    const bool there = key0 < w.n && row_of_16(c, r, kh, key0) >= 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = row16_sum(x[t][i]);
+      const int key = key0 + 4 * qd + i;
+      if (ln == 0 && there && key < w.n) c.weight[rk * c.cap + key] += y;
+    }
+  }
+}
+
+// ---- evict ----------------------------------------------------------------------------------------------------------------------------
+// A workgroup per row and KV head finds the budget-th largest of its keys' ranks (32-bit numbers in the order of the weights, protected keys
+// above all): a histogram over the range that is left, 2048 bins, until a bin is one number -- at most three, mostly of L2 or LDS.  A
+// second launch moves keys and values: with the moves known it spreads over the chip.
+struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
+
+constexpr uint32_t RANK_PROTECTED = 0xffffffffu;
+__device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int recent_from) {
+  if (pos < first || pos >= recent_from) return RANK_PROTECTED;
+  if (w != w) w = -INFINITY;
+  const uint32_t b = __float_as_uint(w + 0.f);                     // (-0 is 0)
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// exclusive sums over the workgroup's 1024 threads of a and b; totals in ta, tb
+__device__ __forceinline__ void block_scan(int& a, int& b, int& ta, int& tb, int2* sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int ia = a, ib = b;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int ua = __shfl_up(ia, o, 64), ub = __shfl_up(ib, o, 64);
+    if (lane >= o) { ia += ua; ib += ub; }
+  }
+  if (lane == 63) sh[wave] = make_int2(ia, ib);
+  __syncthreads();
+  int pa = 0, pb = 0;
+  ta = 0; tb = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const int2 v = sh[w];
+    if (w < wave) { pa += v.x; pb += v.y; }
+    ta += v.x; tb += v.y;
+  }
+  __syncthreads();
+  a = pa + ia - a;
+  b = pb + ib - b;
+}
+
+template <bool IN_LDS>
+__global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, EvictWs ws) {
+  constexpr int BINS = 2048;
+  const int r = blockIdx.y, kh = blockIdx.x, n = held_keys(c, r);
+  const size_t rk = (size_t)r * c.Hkv + kh;
+  if (n <= budget) {
+    if (threadIdx.x == 0) ws.counts[rk] = 0;
+    return;
+  }
+  float* wp = c.weight + rk * c.cap;
+  int32_t* pp = c.pos + rk * c.cap;
+  const int recent_from = c.next[r] - keep_last;
+  extern __shared__ uint32_t ranks[];
+  __shared__ uint32_t hist[BINS];
+  __shared__ int2 scan[16];
+  __shared__ uint32_t sh_lo, sh_hi;
+  __shared__ int sh_prot, sh_bin, sh_above;
+  auto rank = [&](int i) { return IN_LDS ? ranks[i] : rank_of(wp[i], pp[i], keep_first, recent_from); };
+
+  if (threadIdx.x == 0) { sh_lo = 0xffffffffu; sh_hi = 0; sh_prot = 0; }
+  __syncthreads();
+  {
+    uint32_t lo = 0xffffffffu, hi = 0;
+    int prot = 0;
+    for (int i = threadIdx.x; i < n; i += 1024) {
+      const uint32_t k = rank_of(wp[i], pp[i], keep_first, recent_from);
+      if (IN_LDS) ranks[i] = k;
+      if (k == RANK_PROTECTED) ++prot;
+      else { lo = min(lo, k); hi = max(hi, k); }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
+      prot += __shfl_xor(prot, o, 64);
+    }
+    if ((threadIdx.x & 63) == 0) { atomicMin(&sh_lo, lo); atomicMax(&sh_hi, hi); atomicAdd(&sh_prot, prot); }
+  }
+  __syncthreads();
+  // the number `cut` of which some stay: all above it do, of its own the `need` lowest slots
+  uint32_t cut = RANK_PROTECTED;
+  int need = budget;
+  if (sh_prot < budget) {
+    uint32_t lo = sh_lo, hi = sh_hi;
+    need = budget - sh_prot;
+    while (lo != hi) {                                             // the range shrinks by a factor of 1024 at least
+      const int shift = max(0, 21 - __clz(hi - lo));
+      for (int i = threadIdx.x; i < BINS; i += 1024) hist[i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += 1024) {
+        const uint32_t k = rank(i);
+        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+      }
+      __syncthreads();
+      // bins from the highest down, two a thread
+      const int b1 = BINS - 1 - 2 * (int)threadIdx.x, h1 = (int)hist[b1], h0 = (int)hist[b1 - 1];
+      int before = h1 + h0, dummy = 0, t0, t1;
+      block_scan(before, dummy, t0, t1, scan);
+      if (before < need && before + h1 >= need) { sh_bin = b1; sh_above = before; }
+      else if (before + h1 < need && before + h1 + h0 >= need) { sh_bin = b1 - 1; sh_above = before + h1; }
+      __syncthreads();
+      need -= sh_above;
+      lo += (uint32_t)sh_bin << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+    }
+    cut = lo;
+  }
+  // in the order of slots, four a thread and turn: which stay, and the i-th hole in front of `budget` gets the i-th that stays behind it
+  int2* moves = ws.moves + rk * ws.most;
+  int equal0 = 0, holes0 = 0, movers0 = 0;
+  for (int base = 0; base < n; base += 4096) {
+    const int i0 = base + 4 * threadIdx.x;
+    uint32_t k[4];
+    int equal = 0, none = 0, te, tn;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      k[j] = i0 + j < n ? rank(i0 + j) : 0;
+      if (i0 + j < n && k[j] == cut) ++equal;
+    }
+    block_scan(equal, none, te, tn, scan);
+    int at = equal0 + equal, holes = 0, movers = 0, th, tm;
+    bool stays[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      stays[j] = i0 + j < n && (k[j] > cut || (k[j] == cut && at < need));
+      if (i0 + j < n && k[j] == cut) ++at;
+      if (i0 + j < budget && !stays[j]) ++holes;
+      if (i0 + j >= budget && stays[j]) ++movers;
+    }
+    block_scan(holes, movers, th, tm, scan);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j < budget && !stays[j]) moves[holes0 + holes++].y = i0 + j;
+      if (i0 + j >= budget && stays[j]) moves[movers0 + movers++].x = i0 + j;
+    }
+    equal0 += te; holes0 += th; movers0 += tm;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) ws.counts[rk] = movers0;
+  for (int i = threadIdx.x; i < movers0; i += 1024) {
+    const int2 m = moves[i];
+    wp[m.y] = wp[m.x];
+    pp[m.y] = pp[m.x];
+  }
+}
+
+__global__ __launch_bounds__(256) void evict_move_kernel(BoundedCache c, int budget, int row_pieces, EvictWs ws) {
+  const int r = blockIdx.y / c.Hkv, kh = blockIdx.y % c.Hkv;
+  if (blockIdx.x == 0 && kh == 0 && threadIdx.x == 0) c.len[r] = min(held_keys(c, r), budget);       // (nothing else of this launch reads it)
+  const int64_t total = (int64_t)ws.counts[blockIdx.y] * row_pieces;
+  const int2* moves = ws.moves + (size_t)blockIdx.y * ws.most;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+    const int2 m = moves[e / row_pieces];
+    const int p = (int)(e % row_pieces);
+    const int64_t from = row_of_16(c, r, kh, m.x & ~15), to = row_of_16(c, r, kh, m.y & ~15);
+    if (from < 0 || to < 0) continue;
+    const int64_t a = (from + (m.x & 15)) * row_pieces + p, b = (to + (m.y & 15)) * row_pieces + p;
+    ((u32x4*)c.k)[b] = ((const u32x4*)c.k)[a];
+    ((u32x4*)c.v)[b] = ((const u32x4*)c.v)[a];
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------
+
+template <typename F>
+int by_type(int dtype, F&& f) {
+  switch (dtype) {
+    case MI_F32: return f(float{});
+    case MI_BF16: return f(bf16{});
+    case MI_F16: return f(f16{});
+  }
+  return fail(MI_ERR_INVALID, "bounded cache: dtype");
+}
+template <typename F>
+int by_head(int D, F&& f) {                              // (mi_op_bounded_* have looked it over: bounded_head_dim)
+  switch (D) {
+    case 16: return f(std::integral_constant<int, 1>{});
+    case 32: return f(std::integral_constant<int, 2>{});
+    case 64: return f(std::integral_constant<int, 4>{});
+    case 96: return f(std::integral_constant<int, 6>{});
+    case 128: return f(std::integral_constant<int, 8>{});
+    case 192: return f(std::integral_constant<int, 12>{});
+    case 256: return f(std::integral_constant<int, 16>{});
+  }
+  return fail(MI_ERR_UNSUPPORTED, "bounded cache: head_dim");
+}
+
+int attend_splits(const BoundedCache& c, int Hq, int ncu) {
+  const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16);
+  return std::max(1, std::min({MAX_SPLITS, (2 * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
+}
+int weigh_splits(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
+  const int64_t groups = (int64_t)c.rows * c.Hkv * (((int64_t)L * G + STAT_QUERIES - 1) / STAT_QUERIES);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({MAX_SPLITS, 2 * ncu / groups, (c.cap + 255) / 256}));
+}
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+}  // namespace
+
+bool bounded_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
+bool bounded_group(int G) { return G >= 1 && G <= MAX_GROUP; }
+
+size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
+  const size_t splits = attend_splits(c, Hq, ncu), ld = ((size_t)c.cap + 31) & ~(size_t)31;
+  return up256((size_t)c.rows * Hq * ld * 4) + up256((size_t)c.rows * Hq * splits * 8) + up256((size_t)c.rows * Hq * splits * c.D * 4);
+}
+size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  const size_t one = up256((size_t)c.rows * a.Hq * a.L * 8), splits = weigh_splits(c, a, ncu);
+  return splits > 1 ? one * (1 + splits) : one;
+}
+size_t bounded_evict_ws(const BoundedCache& c, int budget) {
+  return up256((size_t)c.rows * c.Hkv * 4) + up256((size_t)c.rows * c.Hkv * std::max(0, std::min(budget, c.cap - budget)) * 8);
+}
+
+int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStream_t st) {
+  int bits = 0;
+  while ((16 << bits) < c.D) ++bits;
+  return by_type(c.dtype, [&](auto z) {
+    using T = decltype(z);
+    if (t.L == 1) {
+      hipLaunchKernelGGL((append_kernel<T, true>), dim3(c.rows), dim3(1024), 0, st, c, t, bits);
+    } else {
+      const int64_t tasks = (int64_t)c.rows * t.L * (t.Hq + 2 * c.Hkv) << bits;
+      hipLaunchKernelGGL((append_kernel<T, false>), dim3((unsigned)((tasks + 255) / 256)), dim3(256), 0, st, c, t, bits);
+      hipLaunchKernelGGL(advance_kernel, dim3((c.rows + 63) / 64), dim3(64), 0, st, c, t);
+    }
+    MI_HIP(hipGetLastError());
+    return MI_OK;
+  });
+}
+
+int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* ws, int ncu, hipStream_t st) {
+  const int splits = attend_splits(c, a.Hq, ncu), G = a.Hq / c.Hkv;
+  AttendWs w;
+  w.ld = (c.cap + 31) & ~31;
+  w.scores = (float*)ws;
+  w.stats = (float*)((char*)ws + up256((size_t)c.rows * a.Hq * w.ld * 4));
+  w.part = (float*)((char*)w.stats + up256((size_t)c.rows * a.Hq * splits * 8));
+  return by_type(c.dtype, [&](auto z) {
+    using T = decltype(z);
+    return by_head(c.D, [&](auto e) {
+      const dim3 grid(splits, c.rows * c.Hkv, (G + 15) / 16);
+      hipLaunchKernelGGL((attend_kernel<T, decltype(e)::value>), grid, dim3(256), 0, st, c, a, w, splits);
+      if (splits > 1 || G > 16)
+        hipLaunchKernelGGL((attend_join_kernel<T>), dim3((c.cap + JOIN_KEYS - 1) / JOIN_KEYS, c.rows * c.Hkv), dim3(256), 0, st, c, a, w, splits);
+      MI_HIP(hipGetLastError());
+      return MI_OK;
+    });
+  });
+}
+
+int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws, int ncu, hipStream_t st) {
+  const int splits = weigh_splits(c, a, ncu), G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
+  const WeighWs w{(float*)ws, (float*)((char*)ws + up256((size_t)c.rows * a.Hq * a.L * 8))};
+  const unsigned rhos = (unsigned)L * G, pairs = c.rows * c.Hkv;
+  return by_type(c.dtype, [&](auto z) {
+    using T = decltype(z);
+    return by_head(c.D, [&](auto e) {
+      constexpr int E = decltype(e)::value;
+      hipLaunchKernelGGL((weigh_stats_kernel<T, E>), dim3((rhos + STAT_QUERIES - 1) / STAT_QUERIES, splits, pairs), dim3(256), 0, st, c, a, w, splits);
+      if (splits > 1) hipLaunchKernelGGL(weigh_merge_kernel, dim3((rhos + 255) / 256, pairs), dim3(256), 0, st, c, a, w, splits);
+      if ((int64_t)((c.cap + 127) / 128) * pairs >= ncu)
+        hipLaunchKernelGGL((weigh_add_kernel<T, E, 2>), dim3((c.cap + 127) / 128, pairs), dim3(256), 0, st, c, a, w);
+      else
+        hipLaunchKernelGGL((weigh_add_kernel<T, E, 1>), dim3((c.cap + 63) / 64, pairs), dim3(256), 0, st, c, a, w);
+      MI_HIP(hipGetLastError());
+      return MI_OK;
+    });
+  });
+}
+
+int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int keep_last, void* ws, hipStream_t st) {
+  if (budget >= c.cap) return MI_OK;                     // no row can hold more
+  const EvictWs w{(int32_t*)ws, (int2*)((char*)ws + up256((size_t)c.rows * c.Hkv * 4)), std::min(budget, c.cap - budget)};
+  const dim3 grid(c.Hkv, c.rows);
+  if (c.cap <= 12288)                                    // ranks in LDS: 48 KiB
+    hipLaunchKernelGGL((evict_select_kernel<true>), grid, dim3(1024), (size_t)c.cap * 4, st, c, budget, keep_first, keep_last, w);
+  else
+    hipLaunchKernelGGL((evict_select_kernel<false>), grid, dim3(1024), 0, st, c, budget, keep_first, keep_last, w);
+  const int pieces = c.D * (int)dtype_size(c.dtype) / 16;
+  const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(64, ((int64_t)w.most * pieces + 1023) / 1024));
+  hipLaunchKernelGGL(evict_move_kernel, dim3(groups, c.rows * c.Hkv), dim3(256), 0, st, c, budget, pieces, w);
+  MI_HIP(hipGetLastError());
+  return MI_OK;
+}
+
+}  // namespace mi

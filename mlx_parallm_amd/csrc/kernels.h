@@ -459,4 +459,42 @@ int launch_rope_tables(float* cos_tab, float* sin_tab, int max_pos, int D, float
                        hipStream_t st);
 int launch_convert(const void* src, int src_dt, void* dst, int dst_dt, size_t n, hipStream_t st);
 
+// ---- a cache of fixed size (bounded.hip; the calls: mi355_ops.h) ----
+struct BoundedCache {
+  int rows, Hkv, D, dtype, cap;
+  int n_blocks, bt_stride, bs_shift;       // paged: btab [rows][bt_stride], blocks of 1 << bs_shift tokens (at least 16)
+  void* k; void* v;                        // [rows][Hkv][cap][D], paged: [n_blocks][Hkv][1 << bs_shift][D]
+  const int32_t* btab;
+  int32_t* len; int32_t* next;             // [rows] slots filled, position of the next token
+  int32_t* pos; float* weight;             // [rows][Hkv][cap]
+};
+struct BoundedTokens {
+  const void* qkv; int64_t ld_row, ld_token;
+  int L, Hq;
+  const int32_t* counts;                   // [rows] tokens that are taken, or null: L
+  const void* q_norm_w; const void* k_norm_w; float eps;
+  const float* cos_tab; const float* sin_tab; int max_pos;
+  void* q_out;                             // [rows][L][Hq][D]
+  // tokens of row r that are taken: what is asked for, as far as there are slots and angles
+  __device__ __forceinline__ int count(const BoundedCache& c, int r, int len, int next) const {
+    const int n = counts != nullptr ? min(counts[r], L) : L;
+    return max(0, next < 0 ? 0 : min(n, min(c.cap - len, max_pos - next)));
+  }
+};
+struct BoundedAttend {
+  const void* q; int Hq; const int32_t* counts; float scale; void* out;       // [rows][Hq][D]; counts: rows with none are left out
+};
+struct BoundedWeigh {
+  const void* q; int L, Hq, last; const int32_t* counts; float scale;         // q [rows][L][Hq][D]
+};
+bool bounded_head_dim(int D);
+bool bounded_group(int G);               // query heads per KV head
+size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu);
+size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu);
+size_t bounded_evict_ws(const BoundedCache& c, int budget);
+int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStream_t st);
+int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* ws, int ncu, hipStream_t st);
+int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws, int ncu, hipStream_t st);
+int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int keep_last, void* ws, hipStream_t st);
+
 }  // namespace mi

@@ -7,6 +7,7 @@
 namespace mi {
 int launch_gemv(const LinearW& W, const GemvCall& c, hipStream_t st);
 bool gemv_mfma_supported(const LinearW& W, const GemvCall& c);
+int gemv_cu_count();
 }  // namespace mi
 
 using namespace mi;
@@ -41,6 +42,35 @@ GemvCall to_call(const mi_op_gemv_args* a) {
   c.force_v1 = a->force_generic;
   return c;
 }
+
+// mi_op_bounded_*: shapes (pointers: false for the sizes of workspaces)
+int bounded_cache(const mi_op_bounded_cache* c, bool pointers, BoundedCache& o) {
+  if (!c) return fail(MI_ERR_INVALID, "null argument");
+  if (c->rows < 1 || c->rows > 65535 || c->Hkv < 1 || c->Hkv > 65535 / c->rows || c->cap < 1 || c->cap > (1 << 30))
+    return fail(MI_ERR_INVALID, "mi_op_bounded: rows, KV heads (at most 65535 together) and slots");
+  if (c->dtype != MI_F32 && c->dtype != MI_BF16 && c->dtype != MI_F16) return fail(MI_ERR_INVALID, "mi_op_bounded: dtype");
+  if (!bounded_head_dim(c->D)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded: head sizes 16, 32, 64, 96, 128, 192 and 256");
+  o = BoundedCache{c->rows, c->Hkv, c->D, c->dtype, c->cap, c->n_blocks, c->bt_stride, c->bs_shift, c->k, c->v, c->btab, c->len, c->next, c->pos, c->weight};
+  if (!pointers) return MI_OK;
+  if (!c->k || !c->v || !c->len || !c->next || !c->pos || !c->weight) return fail(MI_ERR_INVALID, "mi_op_bounded: null array");
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded: keys and values are aligned to 16 bytes");
+  if (c->btab && (c->bs_shift < 4 || c->bs_shift > 20 || c->n_blocks < 1 || c->bt_stride < 1 || (int64_t)c->bt_stride << c->bs_shift < c->cap))
+    return fail(MI_ERR_INVALID, "mi_op_bounded: blocks of a power of two of tokens from 16 on, and a table that reaches to the last slot");
+  return MI_OK;
+}
+
+int bounded_heads(const BoundedCache& c, int Hq) {
+  if (Hq < 1 || Hq % c.Hkv != 0) return fail(MI_ERR_INVALID, "mi_op_bounded: query heads are a multiple of the KV heads");
+  if (!bounded_group(Hq / c.Hkv)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded: at most 128 query heads per KV head");
+  return MI_OK;
+}
+
+int bounded_workspace(const void* ws, uint64_t have, uint64_t need) {
+  if (need && (!ws || (uintptr_t)ws % 16 != 0 || have < need)) return fail(MI_ERR_INVALID, "mi_op_bounded: workspace (its size: the call's _ws)");
+  return MI_OK;
+}
+
+bool bounded_scale(float s) { return s > 0.f && s < INFINITY; }
 
 AttnShape to_shape(const mi_op_attn_shape* s) {
   return AttnShape{s->B, s->L, s->Hq, s->Hkv, s->D, s->act, s->kv, s->rnd, s->cap};
@@ -348,6 +378,75 @@ int mi_op_sample(float* logits, int B, int V, float temperature, float top_p, co
   const int rc = launch_sample(sc, nullptr), rc2 = finish();
   hipFree(sc.ws);
   return rc != MI_OK ? rc : rc2;
+}
+
+int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_tokens* t, void* stream) {
+  BoundedCache b;
+  if (!t) return fail(MI_ERR_INVALID, "null argument");
+  MI_TRY(bounded_cache(c, true, b));
+  MI_TRY(bounded_heads(b, t->Hq));
+  if (t->L < 1 || t->max_pos < 1) return fail(MI_ERR_INVALID, "mi_op_bounded_append: tokens and positions");
+  if (!t->qkv || !t->q_out || !t->cos_tab || !t->sin_tab) return fail(MI_ERR_INVALID, "mi_op_bounded_append: null array");
+  if (!t->q_norm_w != !t->k_norm_w) return fail(MI_ERR_INVALID, "mi_op_bounded_append: the norms of queries and keys go together");
+  if (t->q_norm_w && !(t->eps >= 0.f)) return fail(MI_ERR_INVALID, "mi_op_bounded_append: eps");
+  const uint64_t es = dtype_size(b.dtype);
+  if (((uintptr_t)t->qkv | (uintptr_t)t->q_out | (uintptr_t)t->q_norm_w | (uintptr_t)t->k_norm_w | (uint64_t)t->ld_row * es | (uint64_t)t->ld_token * es) % 16 != 0)
+    return fail(MI_ERR_INVALID, "mi_op_bounded_append: arrays and strides are whole 16 bytes");
+  if ((int64_t)b.rows * t->L > ((int64_t)1 << 31) / (t->Hq + 2 * b.Hkv) * 8) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_append: too many tokens for one call");
+  MI_TRY(ready());
+  return launch_bounded_append(b, BoundedTokens{t->qkv, t->ld_row, t->ld_token, t->L, t->Hq, t->counts, t->q_norm_w, t->k_norm_w, t->eps, t->cos_tab, t->sin_tab,
+                                                t->max_pos, t->q_out}, (hipStream_t)stream);
+}
+
+uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq) {
+  BoundedCache b;
+  return bounded_cache(c, false, b) == MI_OK && bounded_heads(b, Hq) == MI_OK ? bounded_attend_ws(b, Hq, gemv_cu_count()) : 0;
+}
+
+int mi_op_bounded_attend(const mi_op_bounded_cache* c, const void* q, int Hq, const int32_t* counts, float scale, void* out, void* ws, uint64_t ws_bytes, void* stream) {
+  BoundedCache b;
+  MI_TRY(bounded_cache(c, true, b));
+  MI_TRY(bounded_heads(b, Hq));
+  if (!q || !out || (uintptr_t)q % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded_attend: queries (aligned to 16 bytes) and output");
+  if (!bounded_scale(scale)) return fail(MI_ERR_INVALID, "mi_op_bounded_attend: the scale is positive and finite");
+  MI_TRY(ready());
+  MI_TRY(bounded_workspace(ws, ws_bytes, bounded_attend_ws(b, Hq, gemv_cu_count())));
+  return launch_bounded_attend(b, BoundedAttend{q, Hq, counts, scale, out}, ws, gemv_cu_count(), (hipStream_t)stream);
+}
+
+uint64_t mi_op_bounded_weigh_ws(const mi_op_bounded_cache* c, int L, int Hq, int last) {
+  BoundedCache b;
+  if (bounded_cache(c, false, b) != MI_OK || bounded_heads(b, Hq) != MI_OK || L < 1 || last < 0) return 0;
+  return bounded_weigh_ws(b, BoundedWeigh{nullptr, L, Hq, last, nullptr, 1.f}, gemv_cu_count());
+}
+
+int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int Hq, const int32_t* counts, int last, float scale, void* ws, uint64_t ws_bytes,
+                        void* stream) {
+  BoundedCache b;
+  MI_TRY(bounded_cache(c, true, b));
+  MI_TRY(bounded_heads(b, Hq));
+  if (L < 1 || last < 0 || (int64_t)L * Hq > (1 << 30)) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: tokens");
+  if (!q || (uintptr_t)q % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: queries (aligned to 16 bytes)");
+  if (!bounded_scale(scale)) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: the scale is positive and finite");
+  MI_TRY(ready());
+  const BoundedWeigh a{q, L, Hq, last, counts, scale};
+  MI_TRY(bounded_workspace(ws, ws_bytes, bounded_weigh_ws(b, a, gemv_cu_count())));
+  return launch_bounded_weigh(b, a, ws, gemv_cu_count(), (hipStream_t)stream);
+}
+
+uint64_t mi_op_bounded_evict_ws(const mi_op_bounded_cache* c, int budget) {
+  BoundedCache b;
+  return bounded_cache(c, false, b) == MI_OK && budget >= 1 ? bounded_evict_ws(b, budget) : 0;
+}
+
+int mi_op_bounded_evict(const mi_op_bounded_cache* c, int budget, int keep_first, int keep_last, void* ws, uint64_t ws_bytes, void* stream) {
+  BoundedCache b;
+  MI_TRY(bounded_cache(c, true, b));
+  if (budget < 1 || keep_first < 0 || keep_last < 0 || (int64_t)keep_first + keep_last > budget)
+    return fail(MI_ERR_INVALID, "mi_op_bounded_evict: a budget from 1 on that holds the first and last keys that stay");
+  MI_TRY(ready());
+  MI_TRY(bounded_workspace(ws, ws_bytes, bounded_evict_ws(b, budget)));
+  return launch_bounded_evict(b, budget, keep_first, keep_last, ws, (hipStream_t)stream);
 }
 
 }  // extern "C"
