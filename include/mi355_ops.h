@@ -202,9 +202,9 @@ uint64_t mi_op_bounded_weigh_ws(const mi_op_bounded_cache* c, int L, int Hq, int
 int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int Hq, const int32_t* counts, int last, float scale, void* ws, uint64_t ws_bytes,
                         void* stream);
 
-/* At most `budget` keys stay in every row: for each KV head first those at positions below keep_first or among the keep_last before `next`, then by
- * weight (NaN: as -inf), equal ones by the lower slot.  What stays behind slot `budget` moves into the holes in front of it, the i-th into the
- * i-th, with its position and weight; len becomes min(len, budget).  keep_first + keep_last <= budget. */
+/* At most `budget` keys stay in every row: for each KV head those at positions below keep_first or from next - keep_last on before all others, then the more
+ * weighted (NaN: as -inf), equal ones by the lower slot.  What stays behind slot `budget` moves into the holes in front of it, the i-th into the
+ * i-th, with its position and weight; len becomes min(len, budget). */
 uint64_t mi_op_bounded_evict_ws(const mi_op_bounded_cache* c, int budget);
 int mi_op_bounded_evict(const mi_op_bounded_cache* c, int budget, int keep_first, int keep_last, void* ws, uint64_t ws_bytes, void* stream);
 

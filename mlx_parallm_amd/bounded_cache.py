@@ -146,8 +146,8 @@ class BoundedKVCache:
         self._call("mi_op_bounded_weigh", self._ref, q.data_ptr(), q.shape[1], q.shape[2], self._counts(counts), last, self._scale(scale), ws.data_ptr(), n)
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_last: int = 0) -> None:
-        """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last``, then the most
-        weighted, equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it."""
+        """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last`` before all
+        others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it."""
         n = L.lib().mi_op_bounded_evict_ws(self._ref, budget)
         ws = self._workspace(n)
         self._call("mi_op_bounded_evict", self._ref, budget, keep_first, keep_last, ws.data_ptr(), n)

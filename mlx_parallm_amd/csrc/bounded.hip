@@ -654,9 +654,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_a
 // second launch moves keys and values: with the moves known it spreads over the chip.
 struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
 
-constexpr uint32_t RANK_PROTECTED = 0xffffffffu;
-__device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int recent_from) {
-  if (pos < first || pos >= recent_from) return RANK_PROTECTED;
+// Where more keys are protected than the budget holds, they alone are ranked (`crowded`).
+constexpr uint32_t RANK_STAYS = 0xffffffffu, RANK_LEAVES = 0;
+__device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int recent_from, bool crowded) {
+  if ((pos < first || pos >= recent_from) != crowded) return crowded ? RANK_LEAVES : RANK_STAYS;
   if (w != w) w = -INFINITY;
   const uint32_t b = __float_as_uint(w + 0.f);                     // (-0 is 0)
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -697,24 +698,26 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   }
   float* wp = c.weight + rk * c.cap;
   int32_t* pp = c.pos + rk * c.cap;
-  const int recent_from = c.next[r] - keep_last;
+  const int recent_from = (int)max((int64_t)c.next[r] - keep_last, (int64_t)INT32_MIN);
   extern __shared__ uint32_t ranks[];
   __shared__ uint32_t hist[BINS];
   __shared__ int2 scan[16];
   __shared__ uint32_t sh_lo, sh_hi;
   __shared__ int sh_prot, sh_bin, sh_above;
-  auto rank = [&](int i) { return IN_LDS ? ranks[i] : rank_of(wp[i], pp[i], keep_first, recent_from); };
+  bool crowded = false;
+  auto rank = [&](int i) { return IN_LDS ? ranks[i] : rank_of(wp[i], pp[i], keep_first, recent_from, crowded); };
 
-  if (threadIdx.x == 0) { sh_lo = 0xffffffffu; sh_hi = 0; sh_prot = 0; }
-  __syncthreads();
-  {
+  // ranks, their range, and how many keys stay whatever their weight
+  for (int turn = 0; turn < 2; ++turn) {
+    if (threadIdx.x == 0) { sh_lo = 0xffffffffu; sh_hi = 0; sh_prot = 0; }
+    __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0;
     int prot = 0;
     for (int i = threadIdx.x; i < n; i += 1024) {
-      const uint32_t k = rank_of(wp[i], pp[i], keep_first, recent_from);
+      const uint32_t k = rank_of(wp[i], pp[i], keep_first, recent_from, crowded);
       if (IN_LDS) ranks[i] = k;
-      if (k == RANK_PROTECTED) ++prot;
-      else { lo = min(lo, k); hi = max(hi, k); }
+      if (k == RANK_STAYS) ++prot;
+      else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -723,10 +726,13 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
       prot += __shfl_xor(prot, o, 64);
     }
     if ((threadIdx.x & 63) == 0) { atomicMin(&sh_lo, lo); atomicMax(&sh_hi, hi); atomicAdd(&sh_prot, prot); }
+    __syncthreads();
+    if (sh_prot <= budget) break;
+    crowded = true;
+    __syncthreads();
   }
-  __syncthreads();
   // the number `cut` of which some stay: all above it do, of its own the `need` lowest slots
-  uint32_t cut = RANK_PROTECTED;
+  uint32_t cut = RANK_STAYS;
   int need = budget;
   if (sh_prot < budget) {
     uint32_t lo = sh_lo, hi = sh_hi;

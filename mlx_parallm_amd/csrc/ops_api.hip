@@ -442,8 +442,7 @@ uint64_t mi_op_bounded_evict_ws(const mi_op_bounded_cache* c, int budget) {
 int mi_op_bounded_evict(const mi_op_bounded_cache* c, int budget, int keep_first, int keep_last, void* ws, uint64_t ws_bytes, void* stream) {
   BoundedCache b;
   MI_TRY(bounded_cache(c, true, b));
-  if (budget < 1 || keep_first < 0 || keep_last < 0 || (int64_t)keep_first + keep_last > budget)
-    return fail(MI_ERR_INVALID, "mi_op_bounded_evict: a budget from 1 on that holds the first and last keys that stay");
+  if (budget < 1 || keep_first < 0 || keep_last < 0) return fail(MI_ERR_INVALID, "mi_op_bounded_evict: a budget from 1 on, first and last keys from 0 on");
   MI_TRY(ready());
   MI_TRY(bounded_workspace(ws, ws_bytes, bounded_evict_ws(b, budget)));
   return launch_bounded_evict(b, budget, keep_first, keep_last, ws, (hipStream_t)stream);
