@@ -396,7 +396,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 // over S^T = K Q^T: the largest score and the sum of every query (a lane keeps its own over the keys that it holds; four lanes join at the
 // end), then the sum over the queries for every key.  The first keeps queries in registers and passes keys through LDS, the second the
 // other way round.
-struct WeighWs { float* stats; float* parts; };      // [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge
+// Workspace: [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
+// queries, [slice][row][KV head][ld] sums.
+struct WeighWs { float* stats; float* parts; float* sums; int ld; };
 
 struct WeighRow {                                    // what the queries of a row are
   int n, first, queries, behind;                     // keys; first query that asks, their number; query i sees keys up to behind + i
@@ -411,128 +413,214 @@ __device__ __forceinline__ WeighRow weigh_row(const BoundedCache& c, const Bound
   return w;
 }
 
-constexpr int STAT_QUERIES = 128;
 template <typename T, int D>
 constexpr int tile_rows() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }                  // rows of a tile in LDS: two tiles of 16 KiB
 
-// 256 threads hold a tile of ROWS rows in registers on its way from memory to LDS
+// 256 threads hold a tile of ROWS rows in registers on its way from memory to LDS.  Every row has an address (a load under a branch waits for all that
+// are on their way); what is not there is masked where it is used.
 template <typename T, int D, int ROWS>
 struct Stage {
   static constexpr int PER = D * (int)sizeof(T) / 16, LD = D * (int)sizeof(T) + 16;        // pieces a row; bytes a row in LDS (16 more: rows on different banks)
   static constexpr int N = (ROWS * PER + 255) / 256;
   u32x4 w[N];
-  template <typename F>
-  __device__ __forceinline__ void load(F&& row) {                                          // row(i): its address, or null for zeros
-#pragma unroll
-    for (int s = 0; s < N; ++s) {
-      const int p = threadIdx.x + s * 256, i = p / PER;
-      const T* at = ROWS * PER % 256 == 0 || i < ROWS ? row(i) : nullptr;
-      w[s] = at != nullptr ? *(const u32x4*)((const char*)at + p % PER * 16) : u32x4{0, 0, 0, 0};
-    }
-  }
+  static __device__ __forceinline__ int row(int s) { return min((int)(threadIdx.x + s * 256) / PER, ROWS - 1); }      // of this thread's piece s
+  static __device__ __forceinline__ uint32_t piece(int s) { return (threadIdx.x + s * 256) % PER * 16; }              // its bytes in the row
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int s = 0; s < N; ++s) {
-      const int p = threadIdx.x + s * 256, i = p / PER;
-      if (ROWS * PER % 256 == 0 || i < ROWS) *(u32x4*)(lds + i * LD + p % PER * 16) = w[s];
+      const int p = threadIdx.x + s * 256;
+      if (ROWS * PER % 256 == 0 || p < ROWS * PER) *(u32x4*)(lds + p / PER * LD + p % PER * 16) = w[s];
     }
   }
 };
 
-// (float32 heads of 256: one wave a SIMD, or the queries spill)
+// keys that any of the `queries` queries from rho0 on sees
+__device__ __forceinline__ int weigh_most(const WeighRow& w, int G, int rho0, int queries) {
+  return w.behind + w.first + (min(w.queries * G, rho0 + queries) - 1) / G + 1;
+}
+
+// the compiler's order: N times a matrix instruction, then V vector instructions and X exponentials
+template <int N, int V, int X>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+    __builtin_amdgcn_sched_group_barrier(0x400, X, 0);
+  }
+}
+
+// What a workgroup of a pass takes: KV heads side by side (a head stays on one XCD where their number is a multiple of eight), then slices, then tiles, those with
+// the most work first, then rows.  Rows side by side, of unequal lengths, stopped the dispatch: workgroups go round the shader engines in order, so one engine
+// got every workgroup of the longest row and the others waited behind it (4 prompts of up to 2048 tokens: 472 of 1024 places taken for the first 60 us of 88).
+struct WeighPlace { int r, kh, slice, tile; };
+__device__ __forceinline__ WeighPlace weigh_place(const BoundedCache& c, int slices, int tiles) {
+  const int x = blockIdx.x / c.Hkv, y = x / slices;
+  return {y / tiles, (int)(blockIdx.x % c.Hkv), x % slices, y % tiles};
+}
+
+// Queries of a workgroup of the first pass: U tiles of 16 a wave.  16 bits: two (four: 102 us instead of 88 for the pass over 4 prompts of up to 2048 tokens, two waves a SIMD; one: 106);
+// float32, whose tiles cost eight times as much: one (2 prompts of 700 tokens, both passes: 123 us, with two 130).
+template <typename T>
+constexpr int weigh_queries() { return sizeof(T) == 4 ? 64 : 128; }
+
 template <typename T, int E>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_stats_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits) {
-  constexpr int D = 16 * E, ROWS = tile_rows<T, D>();
+__global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_stats_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits, int chunk) {
+  constexpr int D = 16 * E, ROWS = tile_rows<T, D>(), QUERIES = weigh_queries<T>(), U = QUERIES / 64;
   using St = Stage<T, D, ROWS>;
-  const int G = a.Hq / c.Hkv, kh = blockIdx.z % c.Hkv, r = blockIdx.z / c.Hkv, split = blockIdx.y;
+  const int G = a.Hq / c.Hkv;
+  const int qtiles = gridDim.x / (c.rows * c.Hkv * splits);
+  const WeighPlace at = weigh_place(c, splits, qtiles);
+  const int r = at.r, kh = at.kh, split = at.slice;
   const WeighRow w = weigh_row(c, a, r);
-  const int rho0 = (gridDim.x - 1 - blockIdx.x) * STAT_QUERIES, rhos = w.queries * G;      // (the queries that see most keys first)
+  const int rho0 = (qtiles - 1 - at.tile) * QUERIES, rhos = w.queries * G;       // (the queries that see most keys first)
   if (rho0 >= rhos) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
   __shared__ __align__(16) char tiles[2][ROWS * St::LD];
+  __shared__ bool lost[2][ROWS / 16];
 
-  Frag<T, D> q[2];
-  int sees[2];                                           // keys that the column's query sees
+  Frag<T, D> q[U];
+  int sees[U];                                           // keys that the column's query sees
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int rho = rho0 + wave * 32 + u * 16 + ln;
+  for (int u = 0; u < U; ++u) {
+    const int rho = rho0 + (wave * U + u) * 16 + ln;
     const int i = w.first + rho / G, g = rho % G;
     sees[u] = rho < rhos ? w.behind + i + 1 : 0;
     q[u].load((const T*)a.q + (((size_t)r * a.L + min(i, a.L - 1)) * a.Hq + kh * G + g) * D, qd, rho < rhos);
   }
   // the keys of this slice that any query of the workgroup sees, and how many of them all see
-  const int most = w.behind + w.first + (min(rhos, rho0 + STAT_QUERIES) - 1) / G + 1;
-  const int all = rho0 + STAT_QUERIES <= rhos ? w.behind + w.first + rho0 / G + 1 : 0;
-  const int chunk = ((max(most, 0) + splits - 1) / splits + ROWS - 1) / ROWS * ROWS;
+  const int most = weigh_most(w, G, rho0, QUERIES);
+  const int all = rho0 + QUERIES <= rhos ? w.behind + w.first + rho0 / G + 1 : 0;
   const int s0 = split * chunk, s1 = min(most, s0 + chunk);
+  if (s0 >= s1 && split > 0) return;                     // (the merge knows which slices there are)
   const float sc = a.scale * LOG2E;
-  float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
+  float m[U], l[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) { m[u] = -1e30f; l[u] = 0.f; }
   St st;
-  auto fetch = [&](int base) {
-    st.load([&](int i) -> const T* {
-      const int key = base + i;
-      if (key >= s1) return nullptr;
-      const int64_t at = row_of_16(c, r, kh, key & ~15);
-      return at < 0 ? nullptr : (const T*)c.k + (at + (key & 15)) * D;
-    });
+  // Not paged: a tile lies in one piece, behind one address.  Paged: the blocks of the tile after the next one are looked up in time.
+  int block[St::N];
+  bool gone[St::N];
+  const int mask = (1 << c.bs_shift) - 1;
+  const int32_t* table = c.btab != nullptr ? c.btab + (size_t)r * c.bt_stride : nullptr;
+  const char* row0 = (const char*)c.k + ((int64_t)r * c.Hkv + kh) * c.cap * D * (int)sizeof(T);
+  auto look = [&](int base) {
+    if (table == nullptr) return;
+#pragma unroll
+    for (int s = 0; s < St::N; ++s) block[s] = table[min(base + St::row(s), s1 - 1) >> c.bs_shift];
   };
-  if (s0 < s1) { fetch(s0); st.store(tiles[0]); }
+  auto fetch = [&](int base) {
+    if (table == nullptr) {
+      const char* from = row0 + (int64_t)base * D * (int)sizeof(T);
+      const int left = s1 - base;
+      if (left >= ROWS) {
+#pragma unroll
+        for (int s = 0; s < St::N; ++s) st.w[s] = *(const u32x4*)(from + (uint32_t)(St::row(s) * D * (int)sizeof(T) + St::piece(s)));
+      } else {
+#pragma unroll
+        for (int s = 0; s < St::N; ++s) st.w[s] = *(const u32x4*)(from + (uint32_t)(min(St::row(s), left - 1) * D * (int)sizeof(T) + St::piece(s)));
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < St::N; ++s) {
+        gone[s] = (unsigned)block[s] >= (unsigned)c.n_blocks;
+        const int64_t at = (((int64_t)(gone[s] ? 0 : block[s]) * c.Hkv + kh) << c.bs_shift) + (min(base + St::row(s), s1 - 1) & mask);
+        st.w[s] = *(const u32x4*)((const char*)c.k + at * (D * (int)sizeof(T)) + St::piece(s));
+      }
+    }
+  };
+  auto put = [&](int buf) {                              // keys in a block that is none: marked, 16 at a time
+    st.store(tiles[buf]);
+    if (table != nullptr) {
+#pragma unroll
+      for (int s = 0; s < St::N; ++s)
+        if ((threadIdx.x + s * 256) % (16 * St::PER) == 0) lost[buf][St::row(s) / 16] = gone[s];
+    }
+  };
+  if (s0 < s1) {
+    look(s0);
+    fetch(s0);
+    look(s0 + ROWS);
+    put(0);
+  }
   __syncthreads();
   int cur = 0;
   for (int base = s0; base < s1; base += ROWS, cur ^= 1) {
     const bool more = base + ROWS < s1;
-    if (more) fetch(base + ROWS);
+    if (more) {
+      fetch(base + ROWS);
+      look(base + 2 * ROWS);
+    }
     const char* tile = tiles[cur];
-    const bool edge = base + ROWS > min(all, s1) || c.btab != nullptr;
+    bool edge = base + ROWS > min(all, s1);
+    if (table != nullptr) {
 #pragma unroll
-    for (int t0 = 0; t0 < ROWS / 16; t0 += 2) {
-      Frag<T, D> k[2];
-      f32x4 s[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        k[t].load((const T*)(tile + ((t0 + t) * 16 + ln) * St::LD), qd);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s[t][u] = dot16(k[t], q[u]);
-      }
-      if (edge) {
+      for (int t = 0; t < ROWS / 16; ++t) edge = edge || lost[cur][t];
+    }
+    // 32 keys at a time; their products run while the exponentials of the 32 in front of them do
+    auto keys = [&](auto masked) {
+      f32x4 sv[2][2][U];
+      auto products = [&](int t0, f32x4 (&o)[2][U]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int key = base + (t0 + t) * 16;
-          const bool there = c.btab == nullptr || key >= s1 || row_of_16(c, r, kh, key) >= 0;
+          Frag<T, D> k;
+          k.load((const T*)(tile + ((t0 + t) * 16 + ln) * St::LD), qd);
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (key + 4 * qd + i >= min(sees[u], s1) || !there) s[t][u][i] = -INFINITY;
+          for (int u = 0; u < U; ++u) o[t][u] = dot16(k, q[u]);
         }
+      };
+      products(0, sv[0]);
+#pragma unroll
+      for (int t0 = 0; t0 < ROWS / 16; t0 += 2) {
+        if (t0 + 2 < ROWS / 16) products(t0 + 2, sv[(t0 / 2 + 1) & 1]);
+        f32x4 (&s)[2][U] = sv[(t0 / 2) & 1];
+        if constexpr (decltype(masked)::value) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int key = base + (t0 + t) * 16 + 4 * qd;
+            const bool there = table == nullptr || !lost[cur][t0 + t];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int left = there ? min(sees[u], s1) - key : 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (i >= left) s[t][u][i] = -INFINITY;
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float top = s[0][u][0];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i]);
+          top = fmaxf(m[u], top * sc);
+          float x = l[u] * __builtin_amdgcn_exp2f(m[u] - top), y = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x += __builtin_amdgcn_exp2f(fmaf(s[0][u][i], sc, -top));
+            y += __builtin_amdgcn_exp2f(fmaf(s[1][u][i], sc, -top));
+          }
+          m[u] = top; l[u] = x + y;
+        }
+        if constexpr (sizeof(T) == 2 && !decltype(masked)::value) interleave<2 * U * Frag<T, D>::N, 3, 1>();
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float top = m[u];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i] * sc);
-        float x = l[u] * __builtin_amdgcn_exp2f(m[u] - top);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x += __builtin_amdgcn_exp2f(fmaf(s[t][u][i], sc, -top));
-        m[u] = top; l[u] = x;
-      }
-    }
-    if (more) st.store(tiles[cur ^ 1]);
+    };
+    if (edge) keys(std::true_type{});
+    else keys(std::false_type{});
+    if (more) put(cur ^ 1);
     __syncthreads();
   }
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1) {
       const float mo = __shfl_xor(m[u], off, 64), lo = __shfl_xor(l[u], off, 64), M = fmaxf(m[u], mo);
       l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - M) + lo * __builtin_amdgcn_exp2f(mo - M);
       m[u] = M;
     }
-    const int rho = rho0 + wave * 32 + u * 16 + ln;
+    const int rho = rho0 + (wave * U + u) * 16 + ln;
     if (qd == 0 && rho < rhos) {
       const size_t R = (size_t)a.L * G, rk = (size_t)r * c.Hkv + kh;
       if (splits == 1) {
@@ -546,30 +634,54 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_s
   }
 }
 
-__global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits) {
+__global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits, int chunk, int queries) {
   const int G = a.Hq / c.Hkv, r = blockIdx.y / c.Hkv;
   const WeighRow w = weigh_row(c, a, r);
   const int rho = blockIdx.x * 256 + threadIdx.x;
   if (rho >= w.queries * G) return;
   const size_t R = (size_t)a.L * G, rk = blockIdx.y;
+  const int have = max(1, (weigh_most(w, G, rho / queries * queries, queries) + chunk - 1) / chunk);       // slices with keys that the query's workgroups saw
   float M = -1e30f, L = 0.f;
-  for (int i = 0; i < splits; ++i) M = fmaxf(M, ws.parts[((rk * splits + i) * R + rho) * 2]);
-  for (int i = 0; i < splits; ++i) {
-    const float* p = ws.parts + ((rk * splits + i) * R + rho) * 2;
-    L = fmaf(p[1], __builtin_amdgcn_exp2f(p[0] - M), L);
+  for (int i0 = 0; i0 < have; i0 += 8) {               // (eight loads on their way together)
+    float2 p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = *(const float2*)(ws.parts + ((rk * splits + min(i0 + j, have - 1)) * R + rho) * 2);
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j].x);
+    L *= __builtin_amdgcn_exp2f(M - top);
+    M = top;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) L = i0 + j < have ? fmaf(p[j].y, __builtin_amdgcn_exp2f(p[j].x - M), L) : L;
   }
   ws.stats[(rk * R + rho) * 2] = L != 0.f ? M : 0.f;
   ws.stats[(rk * R + rho) * 2 + 1] = L != 0.f ? 1.f / L : 0.f;
 }
 
+// Tiles of the second pass: ROWS queries of one head, those of a head one after the other, from the first query on that sees the workgroup's first
+// key.  A slice is `per` tiles; with more than one of them the sums of each go to the workspace and a third launch adds them in order.
+struct WeighTiles { int i0, per_head, total; };
+__device__ __forceinline__ WeighTiles weigh_tiles(const WeighRow& w, int G, int j0, int rows) {
+  WeighTiles t;
+  t.i0 = max(0, j0 - w.behind - w.first);
+  t.per_head = (max(0, w.queries - t.i0) + rows - 1) / rows;
+  t.total = t.per_head * G;
+  return t;
+}
+
 template <typename T, int E, int KS>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_add_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_add_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int per, int slices) {
   constexpr int D = 16 * E, ROWS = tile_rows<T, D>();
   using St = Stage<T, D, ROWS>;
-  const int G = a.Hq / c.Hkv, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
+  const int G = a.Hq / c.Hkv;
+  const WeighPlace at = weigh_place(c, slices, gridDim.x / (c.rows * c.Hkv * slices));
+  const int r = at.r, kh = at.kh;
   const WeighRow w = weigh_row(c, a, r);
-  const int j0 = blockIdx.x * 64 * KS;
-  if (j0 >= w.n || w.queries <= 0) return;
+  const int j0 = at.tile * 64 * KS;
+  if (j0 >= w.n) return;
+  const WeighTiles wt = weigh_tiles(w, G, j0, ROWS);
+  const int t0 = at.slice * per, t1 = min(wt.total, t0 + per);
+  if (t0 >= t1) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
   __shared__ __align__(16) char tiles[2][ROWS * St::LD];
   __shared__ float2 stats[2][ROWS];
@@ -579,13 +691,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_a
 #pragma unroll
   for (int t = 0; t < KS; ++t) {
     const int key = my0 + 16 * t;
-    const int64_t at = key < w.n ? row_of_16(c, r, kh, key) : -1;
-    k[t].load((const T*)c.k + ((at < 0 ? 0 : at) + min(ln, max(0, w.n - 1 - key))) * D, qd, at >= 0);
+    const int64_t row = key < w.n ? row_of_16(c, r, kh, key) : -1;
+    k[t].load((const T*)c.k + ((row < 0 ? 0 : row) + min(ln, max(0, w.n - 1 - key))) * D, qd, row >= 0);
   }
-  const int rhos = w.queries * G;
-  const int from = max(0, j0 - w.behind - w.first) * G;            // the first query that sees key j0
   const float sc = a.scale * LOG2E;
-  const size_t R = (size_t)a.L * G, rk = (size_t)r * c.Hkv + kh;
+  const size_t rk = (size_t)r * c.Hkv + kh;
+  const float* st_row = ws.stats + rk * a.L * G * 2;
+  const T* q_row = (const T*)a.q + (((size_t)r * a.L + w.first) * a.Hq + kh * G) * D;
+  const int64_t ld_q = (int64_t)a.Hq * D;
   float x[KS][4];
 #pragma unroll
   for (int t = 0; t < KS; ++t)
@@ -593,42 +706,64 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_a
     for (int i = 0; i < 4; ++i) x[t][i] = 0.f;
   St st;
   float2 sv = make_float2(0.f, 0.f);
-  auto fetch = [&](int base) {
-    st.load([&](int i) -> const T* {
-      const int rho = base + i;
-      return rho < rhos ? (const T*)a.q + (((size_t)r * a.L + w.first + rho / G) * a.Hq + kh * G + rho % G) * D : nullptr;
-    });
-    if (threadIdx.x < ROWS) sv = base + (int)threadIdx.x < rhos ? *(const float2*)(ws.stats + (rk * R + base + threadIdx.x) * 2) : make_float2(0.f, 0.f);
+  uint32_t off[St::N];                                 // of this thread's pieces from a tile's first row
+#pragma unroll
+  for (int s = 0; s < St::N; ++s) off[s] = (uint32_t)(St::row(s) * ld_q * sizeof(T)) + St::piece(s);
+  auto fetch = [&](int g, int first) {                 // queries first .. first + ROWS of head g; the last one again behind it, where it weighs nothing
+    const int left = w.queries - first;
+    const char* from = (const char*)(q_row + first * ld_q + g * D);
+    const float* stat = st_row + ((size_t)first * G + g) * 2;
+    if (left >= ROWS) {
+#pragma unroll
+      for (int s = 0; s < St::N; ++s) st.w[s] = *(const u32x4*)(from + off[s]);
+      sv = *(const float2*)(stat + (threadIdx.x % ROWS) * G * 2);
+    } else {
+#pragma unroll
+      for (int s = 0; s < St::N; ++s) st.w[s] = *(const u32x4*)(from + min((int64_t)St::row(s), (int64_t)left - 1) * ld_q * sizeof(T) + St::piece(s));
+      sv = *(const float2*)(stat + min((int)threadIdx.x % ROWS, left - 1) * G * 2);
+      if ((int)threadIdx.x >= left) sv = make_float2(1e30f, 0.f);
+    }
   };
-  if (from < rhos) {
-    fetch(from);
-    st.store(tiles[0]);
-    if (threadIdx.x < ROWS) stats[0][threadIdx.x] = sv;
-  }
+  int g = t0 / wt.per_head, it = t0 % wt.per_head;
+  fetch(g, wt.i0 + it * ROWS);
+  st.store(tiles[0]);
+  if (threadIdx.x < ROWS) stats[0][threadIdx.x] = sv;
   __syncthreads();
   int cur = 0;
-  for (int base = from; base < rhos; base += ROWS, cur ^= 1) {
-    const bool more = base + ROWS < rhos;
-    if (more) fetch(base + ROWS);
+  for (int tt = t0; tt < t1; ++tt, cur ^= 1) {
+    const int first = wt.i0 + it * ROWS;
+    if (++it == wt.per_head) { it = 0; ++g; }
+    const bool more = tt + 1 < t1;
+    if (more) fetch(g, wt.i0 + it * ROWS);
     const char* tile = tiles[cur];
-    const bool edge = w.behind + w.first + base / G + 1 < my0 + 16 * KS;      // the tile's first query does not see all keys of this wave
+    const int sees0 = w.behind + w.first + first + 1;    // keys that the tile's first query sees
+    // the products of 16 queries run while the exponentials of the 16 in front of them do
+    auto columns = [&](auto edge) {
+      f32x4 sv2[2][KS];
+      auto products = [&](int u, f32x4 (&o)[KS]) {
+        Frag<T, D> q;
+        q.load((const T*)(tile + (u * 16 + ln) * St::LD), qd);
 #pragma unroll
-    for (int u = 0; u < ROWS / 16; ++u) {
-      Frag<T, D> q;
-      q.load((const T*)(tile + (u * 16 + ln) * St::LD), qd);
-      const float2 ml = stats[cur][u * 16 + ln];
-      const int sees = w.behind + w.first + (base + u * 16 + ln) / G + 1;
+        for (int t = 0; t < KS; ++t) o[t] = dot16(k[t], q);
+      };
+      products(0, sv2[0]);
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        const f32x4 s = dot16(k[t], q);
+      for (int u = 0; u < ROWS / 16; ++u) {
+        if (u + 1 < ROWS / 16) products(u + 1, sv2[(u + 1) & 1]);
+        const float2 ml = stats[cur][u * 16 + ln];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[i], sc, -ml.x));
-          if (edge && my0 + 16 * t + 4 * qd + i >= sees) p = 0.f;
-          x[t][i] = fmaf(p, ml.y, x[t][i]);
-        }
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p = __builtin_amdgcn_exp2f(fmaf(sv2[u & 1][t][i], sc, -ml.x));
+            if (decltype(edge)::value && my0 + 16 * t + 4 * qd + i >= sees0 + u * 16 + ln) p = 0.f;
+            x[t][i] = fmaf(p, ml.y, x[t][i]);
+          }
+        if constexpr (sizeof(T) == 2) interleave<KS * Frag<T, D>::N, 2, 1>();
       }
-    }
+    };
+    if (sees0 < my0 + 16 * KS) columns(std::true_type{});
+    else columns(std::false_type{});
     if (more) {
       st.store(tiles[cur ^ 1]);
       if (threadIdx.x < ROWS) stats[cur ^ 1][threadIdx.x] = sv;
@@ -643,9 +778,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && E > 12 ? 1 : 2) void weigh_a
     for (int i = 0; i < 4; ++i) {
       const float y = row16_sum(x[t][i]);
       const int key = key0 + 4 * qd + i;
-      if (ln == 0 && there && key < w.n) c.weight[rk * c.cap + key] += y;
+      if (ln != 0 || key >= w.n) continue;
+      if (slices > 1) ws.sums[((size_t)at.slice * c.rows * c.Hkv + rk) * ws.ld + key] = there ? y : 0.f;
+      else if (there) c.weight[rk * c.cap + key] += y;
     }
   }
+}
+
+__global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int per, int keys, int rows) {
+  const int G = a.Hq / c.Hkv, r = blockIdx.y / c.Hkv, key = blockIdx.x * 256 + threadIdx.x;
+  const WeighRow w = weigh_row(c, a, r);
+  if (key >= w.n) return;
+  const int slices = (weigh_tiles(w, G, key / keys * keys, rows).total + per - 1) / per;
+  const float* p = ws.sums + (size_t)blockIdx.y * ws.ld + key;
+  const size_t step = (size_t)c.rows * c.Hkv * ws.ld;
+  float x = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < slices; ++i) x += p[i * step];
+  if (slices > 0) c.weight[(size_t)blockIdx.y * c.cap + key] += x;
 }
 
 // ---- evict ----------------------------------------------------------------------------------------------------------------------------
@@ -843,10 +993,24 @@ int attend_splits(const BoundedCache& c, int Hq, int ncu) {
   const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16);
   return std::max(1, std::min({MAX_SPLITS, (2 * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
 }
-int weigh_splits(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
-  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
-  const int64_t groups = (int64_t)c.rows * c.Hkv * (((int64_t)L * G + STAT_QUERIES - 1) / STAT_QUERIES);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({MAX_SPLITS, 2 * ncu / groups, (c.cap + 255) / 256}));
+// How a call is cut: units of nearly equal size, several times as many as the chip holds at once, so that its queues even them out.  First pass: 64 U queries by
+// `chunk` keys; second: 64 KS keys by `per` tiles of queries.
+struct WeighPlan { int splits, chunk, ks, per, slices; };
+WeighPlan weigh_plan(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  WeighPlan p;
+  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L, f32 = c.dtype == MI_F32, U = f32 ? 1 : 2;
+  const int64_t pairs = (int64_t)c.rows * c.Hkv, groups = pairs * (((int64_t)L * G + 64 * U - 1) / (64 * U));
+  const int64_t fit = std::max<int64_t>({(int64_t)c.cap * groups / ((f32 ? 16 : 8) * ncu), 256, (c.cap + MAX_SPLITS - 1) / MAX_SPLITS});
+  p.chunk = (int)std::min<int64_t>((fit + 63) / 64 * 64, (c.cap + 63) / 64 * 64);
+  p.splits = (c.cap + p.chunk - 1) / p.chunk;
+  auto key_tiles = [&](int ks) { return pairs * ((c.cap + 64 * ks - 1) / (64 * ks)); };
+  p.ks = !f32 && key_tiles(2) >= ncu ? 2 : 1;
+  const int rows = c.D * (int)dtype_size(c.dtype) <= 256 ? 64 : 32;
+  const int64_t tiles = (int64_t)G * ((L + rows - 1) / rows), least = f32 ? 4 : 8;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({MAX_SPLITS, 24 * ncu / key_tiles(p.ks), (tiles + least - 1) / least}));
+  p.per = (int)((tiles + want - 1) / want);
+  p.slices = (int)((tiles + p.per - 1) / p.per);
+  return p;
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -861,8 +1025,9 @@ size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
   return up256((size_t)c.rows * Hq * ld * 4) + up256((size_t)c.rows * Hq * splits * 8) + up256((size_t)c.rows * Hq * splits * c.D * 4);
 }
 size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
-  const size_t one = up256((size_t)c.rows * a.Hq * a.L * 8), splits = weigh_splits(c, a, ncu);
-  return splits > 1 ? one * (1 + splits) : one;
+  const WeighPlan p = weigh_plan(c, a, ncu);
+  const size_t one = up256((size_t)c.rows * a.Hq * a.L * 8), ld = ((size_t)c.cap + 3) & ~(size_t)3;
+  return one + std::max(p.splits > 1 ? one * p.splits : 0, p.slices > 1 ? (size_t)p.slices * c.rows * c.Hkv * ld * 4 : 0);
 }
 size_t bounded_evict_ws(const BoundedCache& c, int budget) {
   return up256((size_t)c.rows * c.Hkv * 4) + up256((size_t)c.rows * c.Hkv * std::max(0, std::min(budget, c.cap - budget)) * 8);
@@ -906,19 +1071,23 @@ int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* w
 }
 
 int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws, int ncu, hipStream_t st) {
-  const int splits = weigh_splits(c, a, ncu), G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
-  const WeighWs w{(float*)ws, (float*)((char*)ws + up256((size_t)c.rows * a.Hq * a.L * 8))};
+  const WeighPlan p = weigh_plan(c, a, ncu);
+  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
+  float* more = (float*)((char*)ws + up256((size_t)c.rows * a.Hq * a.L * 8));
+  const WeighWs w{(float*)ws, more, more, (c.cap + 3) & ~3};
   const unsigned rhos = (unsigned)L * G, pairs = c.rows * c.Hkv;
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
     return by_head(c.D, [&](auto e) {
       constexpr int E = decltype(e)::value;
-      hipLaunchKernelGGL((weigh_stats_kernel<T, E>), dim3((rhos + STAT_QUERIES - 1) / STAT_QUERIES, splits, pairs), dim3(256), 0, st, c, a, w, splits);
-      if (splits > 1) hipLaunchKernelGGL(weigh_merge_kernel, dim3((rhos + 255) / 256, pairs), dim3(256), 0, st, c, a, w, splits);
-      if ((int64_t)((c.cap + 127) / 128) * pairs >= ncu)
-        hipLaunchKernelGGL((weigh_add_kernel<T, E, 2>), dim3((c.cap + 127) / 128, pairs), dim3(256), 0, st, c, a, w);
-      else
-        hipLaunchKernelGGL((weigh_add_kernel<T, E, 1>), dim3((c.cap + 63) / 64, pairs), dim3(256), 0, st, c, a, w);
+      constexpr int Q = weigh_queries<T>(), KS = sizeof(T) == 4 ? 1 : 2;
+      const dim3 queries((rhos + Q - 1) / Q * p.splits * pairs), keys((c.cap + 64 * p.ks - 1) / (64 * p.ks) * p.slices * pairs);
+      hipLaunchKernelGGL((weigh_stats_kernel<T, E>), queries, dim3(256), 0, st, c, a, w, p.splits, p.chunk);
+      if (p.splits > 1) hipLaunchKernelGGL(weigh_merge_kernel, dim3((rhos + 255) / 256, pairs), dim3(256), 0, st, c, a, w, p.splits, p.chunk, Q);
+      if (p.ks == KS) hipLaunchKernelGGL((weigh_add_kernel<T, E, KS>), keys, dim3(256), 0, st, c, a, w, p.per, p.slices);
+      else hipLaunchKernelGGL((weigh_add_kernel<T, E, 1>), keys, dim3(256), 0, st, c, a, w, p.per, p.slices);
+      if (p.slices > 1)
+        hipLaunchKernelGGL(weigh_sum_kernel, dim3((c.cap + 255) / 256, pairs), dim3(256), 0, st, c, a, w, p.per, 64 * p.ks, tile_rows<T, 16 * E>());
       MI_HIP(hipGetLastError());
       return MI_OK;
     });

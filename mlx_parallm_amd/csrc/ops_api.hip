@@ -61,7 +61,7 @@ int bounded_cache(const mi_op_bounded_cache* c, bool pointers, BoundedCache& o) 
 
 int bounded_heads(const BoundedCache& c, int Hq) {
   if (Hq < 1 || Hq % c.Hkv != 0) return fail(MI_ERR_INVALID, "mi_op_bounded: query heads are a multiple of the KV heads");
-  if (!bounded_group(Hq / c.Hkv)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded: at most 128 query heads per KV head");
+  if (Hq > 8192 || !bounded_group(Hq / c.Hkv)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded: at most 128 query heads per KV head, 8192 in all");
   return MI_OK;
 }
 
@@ -425,7 +425,8 @@ int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int 
   BoundedCache b;
   MI_TRY(bounded_cache(c, true, b));
   MI_TRY(bounded_heads(b, Hq));
-  if (L < 1 || last < 0 || (int64_t)L * Hq > (1 << 30)) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: tokens");
+  if (L < 1 || last < 0) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: tokens");
+  if ((int64_t)b.rows * L > ((int64_t)1 << 31) / Hq) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_weigh: too many tokens for one call");
   if (!q || (uintptr_t)q % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: queries (aligned to 16 bytes)");
   if (!bounded_scale(scale)) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: the scale is positive and finite");
   MI_TRY(ready());
