@@ -28,6 +28,9 @@ from . import _lib as L
 _DTYPES = {torch.float32: L.MI_F32, torch.bfloat16: L.MI_BF16, torch.float16: L.MI_F16}
 _NAMES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 
+# the current stream's handle: a tenth of a microsecond, where torch.cuda.current_stream() makes an object for it in 2.7 -- a fifth of a short call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
@@ -64,7 +67,7 @@ class BoundedKVCache:
         self.keys, self.values, self.lengths, self.next_positions = keys, values, lengths, next_positions
         self.positions, self.weights, self.block_table = positions, weights, block_table
         self.rows, self.kv_heads, self.capacity, self.head_dim = rows, heads, cap, keys.shape[3]
-        self.dtype, self.device = keys.dtype, keys.device
+        self.dtype, self.device, self._index = keys.dtype, keys.device, keys.device.index
         c = L.OpBoundedCache()
         c.rows, c.Hkv, c.D, c.dtype, c.cap = rows, heads, self.head_dim, _DTYPES[keys.dtype], cap
         if block_table is not None:
@@ -74,8 +77,7 @@ class BoundedKVCache:
             c.n_blocks, c.bt_stride, c.bs_shift = keys.shape[0], block_table.shape[1], tokens.bit_length() - 1
         c.k, c.v, c.btab = keys.data_ptr(), values.data_ptr(), _ptr(block_table)
         c.len, c.next, c.pos, c.weight = lengths.data_ptr(), next_positions.data_ptr(), positions.data_ptr(), weights.data_ptr()
-        self._c = c
-        self._ref = C.byref(c)
+        self._c, self._ref, self._lib = c, C.byref(c), L.lib()
 
     @classmethod
     def create(cls, rows: int, kv_heads: int, head_dim: int, capacity: int, dtype="bfloat16", *, block_tokens: int = 0, device="cuda") -> "BoundedKVCache":
@@ -98,26 +100,24 @@ class BoundedKVCache:
         [rows, L, heads, head_dim], normed (where ``q_norm`` / ``k_norm`` [head_dim] are given) and rotated by ``cos`` / ``sin``
         [positions, head_dim / 2] float32.  ``counts`` [rows] int32: row r takes its first counts[r] tokens, the queries of the others are zeros.  A row
         takes no more than it has slots and the tables have positions."""
-        D = self.head_dim
+        D, f32 = self.head_dim, torch.float32
         self._check(qkv, "qkv", self.dtype)
-        if qkv.dim() != 3 or qkv.shape[0] != self.rows or qkv.shape[1] < 1 or qkv.shape[2] != (heads + 2 * self.kv_heads) * D or qkv.stride(2) != 1:
+        rows, tokens, width = qkv.shape if qkv.dim() == 3 else (0, 0, 0)
+        if rows != self.rows or tokens < 1 or width != (heads + 2 * self.kv_heads) * D or qkv.stride(2) != 1:
             raise ValueError(f"qkv: [{self.rows}, tokens, {(heads + 2 * self.kv_heads) * D}], contiguous in the last dimension")
-        for t, what in ((cos, "cos"), (sin, "sin")):
-            self._check(t, what, torch.float32)
-            if t.dim() != 2 or t.shape != cos.shape or t.shape[1] != D // 2 or not t.is_contiguous():
-                raise ValueError(f"{what}: [positions, {D // 2}], contiguous")
+        self._check(cos, "cos", f32)
+        self._check(sin, "sin", f32)
+        if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError(f"cos, sin: [positions, {D // 2}], contiguous")
         for t in (q_norm, k_norm):
             if t is not None:
                 self._check(t, "norm weights", self.dtype)
-                if tuple(t.shape) != (D,) or not t.is_contiguous():
+                if t.shape != (D,) or not t.is_contiguous():
                     raise ValueError(f"norm weights: [{D}]")
-        a = L.OpBoundedTokens()
-        a.qkv, a.ld_row, a.ld_token, a.L, a.Hq = qkv.data_ptr(), qkv.stride(0), qkv.stride(1), qkv.shape[1], heads
-        a.counts, a.q_norm_w, a.k_norm_w, a.eps = self._counts(counts), _ptr(q_norm), _ptr(k_norm), eps
-        a.max_pos, a.cos_tab, a.sin_tab = cos.shape[0], cos.data_ptr(), sin.data_ptr()
-        q = torch.empty((self.rows, qkv.shape[1], heads, D), dtype=self.dtype, device=self.device)
-        a.q_out = q.data_ptr()
-        self._call("mi_op_bounded_append", self._ref, C.byref(a))
+        q = qkv.new_empty((rows, tokens, heads, D))
+        a = L.OpBoundedTokens(qkv.data_ptr(), qkv.stride(0), qkv.stride(1), tokens, heads, self._counts(counts), _ptr(q_norm), _ptr(k_norm), eps, cos.shape[0],
+                              cos.data_ptr(), sin.data_ptr(), q.data_ptr())
+        self._call(self._lib.mi_op_bounded_append, self._ref, C.byref(a))
         return q
 
     def attend(self, q, scale: Optional[float] = None, *, counts=None):
@@ -129,9 +129,9 @@ class BoundedKVCache:
         q = q.contiguous()
         heads = q.shape[1]
         out = torch.empty_like(q)
-        n = L.lib().mi_op_bounded_attend_ws(self._ref, heads)
+        n = self._lib.mi_op_bounded_attend_ws(self._ref, heads)
         ws = self._workspace(n)
-        self._call("mi_op_bounded_attend", self._ref, q.data_ptr(), heads, self._counts(counts), self._scale(scale), out.data_ptr(), ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_attend, self._ref, q.data_ptr(), heads, self._counts(counts), self._scale(scale), out.data_ptr(), ws.data_ptr(), n)
         return out
 
     def weigh(self, q, scale: Optional[float] = None, *, counts=None, last: int = 0) -> None:
@@ -141,16 +141,16 @@ class BoundedKVCache:
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != self.head_dim:
             raise ValueError(f"q: [{self.rows}, tokens, heads, {self.head_dim}]")
         q = q.contiguous()
-        n = L.lib().mi_op_bounded_weigh_ws(self._ref, q.shape[1], q.shape[2], last)
+        n = self._lib.mi_op_bounded_weigh_ws(self._ref, q.shape[1], q.shape[2], last)
         ws = self._workspace(n)
-        self._call("mi_op_bounded_weigh", self._ref, q.data_ptr(), q.shape[1], q.shape[2], self._counts(counts), last, self._scale(scale), ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_weigh, self._ref, q.data_ptr(), q.shape[1], q.shape[2], self._counts(counts), last, self._scale(scale), ws.data_ptr(), n)
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_last: int = 0) -> None:
         """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last`` before all
         others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it."""
-        n = L.lib().mi_op_bounded_evict_ws(self._ref, budget)
+        n = self._lib.mi_op_bounded_evict_ws(self._ref, budget)
         ws = self._workspace(n)
-        self._call("mi_op_bounded_evict", self._ref, budget, keep_first, keep_last, ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_evict, self._ref, budget, keep_first, keep_last, ws.data_ptr(), n)
 
     def reset(self) -> None:
         """Every row empty, its next token at position 0."""
@@ -167,7 +167,7 @@ class BoundedKVCache:
         if t is None:
             return None
         self._check(t, "counts", torch.int32)
-        if tuple(t.shape) != (self.rows,) or not t.is_contiguous():
+        if t.shape != (self.rows,) or not t.is_contiguous():
             raise ValueError("counts: one number a row")
         return t.data_ptr()
 
@@ -176,14 +176,15 @@ class BoundedKVCache:
 
     def _workspace(self, n: int):
         # of torch's allocator, call by call: its blocks go round in the order of the stream, and a captured graph has its own
-        return torch.empty(n, dtype=torch.uint8, device=self.device)
+        return self.lengths.new_empty((n + 3) // 4)
 
-    def _call(self, name: str, *args) -> None:
+    def _call(self, fn, *args) -> None:
         if self.device.type != "cuda":
             raise RuntimeError("no HIP device: the cache's tensors are on " + str(self.device))
-        fn = getattr(L.lib(), name)
-        if torch.cuda.current_device() == self.device.index:
-            L.check(fn(*args, torch.cuda.current_stream().cuda_stream))
-            return
-        with torch.cuda.device(self.device):
-            L.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        if torch.cuda.current_device() == self._index:
+            rc = fn(*args, _raw_stream(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                rc = fn(*args, _raw_stream(self._index))
+        if rc:
+            L.check(rc)

@@ -63,21 +63,23 @@ __device__ __forceinline__ Raw<NB> load_bits(const void* p) {
 // ---- append ---------------------------------------------------------------------------------------------------------------------------
 // One lane takes 8 + 8 elements of a head, i .. i + 8 and i + D / 2 .. i + D / 2 + 8 (the two halves of a rotation's pairs), a power of two of
 // lanes a head.  All in 32 bits, rounded once, to what is stored.
-// STEP (one token a row): a workgroup per row, which moves the row's length and next position itself.  Otherwise the tasks of all tokens lie
+// STEP (few tokens a row): a workgroup per row, which moves the row's length and next position itself.  Otherwise the tasks of all tokens lie
 // side by side and a second launch moves them.
 template <typename T>
 struct alignas(16) Vec8 { T v[8]; };
+
+constexpr int STEP_TASKS = 8192;
 
 template <typename T, bool STEP>
 __global__ __launch_bounds__(STEP ? 1024 : 256) void append_kernel(BoundedCache c, BoundedTokens t, int lane_bits) {
   const int nh = t.Hq + 2 * c.Hkv, D = c.D, D2 = D / 2, lanes = 1 << lane_bits;
   const int per_token = nh << lane_bits;
-  const int64_t total = STEP ? per_token : (int64_t)c.rows * t.L * per_token;
+  const int64_t total = (STEP ? 1 : (int64_t)c.rows) * t.L * per_token;
   int n_step = 0, len_step = 0, next_step = 0;
   for (int64_t task = STEP ? threadIdx.x : (int64_t)blockIdx.x * 256 + threadIdx.x; task < total; task += STEP ? 1024 : total) {
-    const int64_t token = STEP ? blockIdx.x : task / per_token;
-    const int in_token = (int)(STEP ? task : task - token * per_token);
-    const int r = (int)(token / t.L), i = (int)(token - (int64_t)r * t.L);
+    const int64_t token = (STEP ? (int64_t)blockIdx.x * t.L : 0) + (t.L == 1 && STEP ? 0 : STEP ? (uint32_t)task / (uint32_t)per_token : task / per_token);
+    const int in_token = (int)(STEP ? (t.L == 1 ? task : (uint32_t)task % (uint32_t)per_token) : task % per_token);
+    const int r = STEP ? blockIdx.x : (int)(token / t.L), i = (int)(token - (int64_t)r * t.L);
     const int head = in_token >> lane_bits, e0 = (in_token & (lanes - 1)) * 8;
     const int len = held_keys(c, r), next = c.next[r];
     const int n = t.count(c, r, len, next);
@@ -352,42 +354,69 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
   }
 }
 
-// The slices' results joined: the output, and the weights of JOIN_KEYS keys a workgroup.
+// The slices' results joined: the output, and the weights of JOIN_KEYS keys a workgroup, four a thread.  What depends on no result -- the scores of the first
+// heads -- is on its way before the statistics are.
 constexpr int JOIN_KEYS = 1024;
 
 template <typename T>
 __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
+  constexpr int HB = 4;                                 // heads whose scores are loaded together
   const int G = a.Hq / c.Hkv, D = c.D, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
   const bool idle = a.counts != nullptr && a.counts[r] <= 0;
   const int n = idle ? 0 : held_keys(c, r);
   if (blockIdx.x > 0 && (int)blockIdx.x * JOIN_KEYS >= n) return;
   const int chunk = slice_keys(n, splits), ns = n > 0 ? (n + chunk - 1) / chunk : 0;
+  const int key = blockIdx.x * JOIN_KEYS + 4 * threadIdx.x;
+  const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld + min(key, max(0, ws.ld - 4));
+  f32x4 s[HB];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int j = 0; j < HB; ++j) s[j] = *(const f32x4*)(sp + (size_t)min(h0 + j, G - 1) * ws.ld);
+  };
+  fetch(0);
   __shared__ float sh_m[MAX_GROUP], sh_r[MAX_GROUP];
   const float* st = ws.stats + (size_t)(r * c.Hkv + kh) * splits * G * 2;
   for (int h = threadIdx.x >> 6; h < G; h += 4) {       // a wave per head, a lane per slice
     const int i = threadIdx.x & 63;
-    const float m = i < ns ? st[((size_t)i * G + h) * 2] : -1e30f, M = wave_max(m);
-    const float L = wave_sum(i < ns ? st[((size_t)i * G + h) * 2 + 1] * __builtin_amdgcn_exp2f(m - M) : 0.f);
+    const float2 v = ns > 0 ? *(const float2*)(st + ((size_t)min(i, ns - 1) * G + h) * 2) : make_float2(-1e30f, 0.f);
+    const float M = wave_max(v.x), L = wave_sum(i < ns ? v.y * __builtin_amdgcn_exp2f(v.x - M) : 0.f);
     if (i == 0) { sh_m[h] = M; sh_r[h] = L != 0.f ? 1.f / L : 0.f; }
   }
   __syncthreads();
+  if (key < n) {
+    const float sc = a.scale * LOG2E;
+    f32x4 x{0.f, 0.f, 0.f, 0.f};
+    for (int h0 = 0; h0 < G; h0 += HB) {
+      if (h0 > 0) fetch(h0);
+#pragma unroll
+      for (int j = 0; j < HB; ++j)
+        if (h0 + j < G)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[j][i], sc, -sh_m[h0 + j])), sh_r[h0 + j], x[i]);
+    }
+    float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap + key;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key + i < n) wp[i] += x[i];
+  }
   // the output: its elements spread over the row's workgroups
   const int groups = max(1, (n + JOIN_KEYS - 1) / JOIN_KEYS);
   const float* pp = ws.part + (size_t)(r * c.Hkv + kh) * splits * G * D;
   for (int e = blockIdx.x * 256 + threadIdx.x; e < G * D; e += groups * 256) {
     const int h = e / D;
     float x = 0.f;
-    for (int i = 0; i < ns; ++i) x = fmaf(pp[(size_t)i * G * D + e], __builtin_amdgcn_exp2f(st[((size_t)i * G + h) * 2] - sh_m[h]), x);
+    for (int i0 = 0; i0 < ns; i0 += 8) {
+      float o[8], m[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const size_t i = (size_t)min(i0 + j, ns - 1) * G;
+        o[j] = pp[i * D + e];
+        m[j] = st[(i + h) * 2];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], __builtin_amdgcn_exp2f(m[j] - sh_m[h]), x) : x;
+    }
     ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
-  }
-  const float sc = a.scale * LOG2E;
-  const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld;
-  float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
-  const int k0 = blockIdx.x * JOIN_KEYS;
-  for (int key = k0 + threadIdx.x; key < min(n, k0 + JOIN_KEYS); key += 256) {
-    float x = 0.f;
-    for (int h = 0; h < G; ++h) x = fmaf(__builtin_amdgcn_exp2f(fmaf(sp[(size_t)h * ws.ld + key], sc, -sh_m[h])), sh_r[h], x);
-    wp[key] += x;
   }
 }
 
@@ -800,7 +829,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 
 // ---- evict ----------------------------------------------------------------------------------------------------------------------------
 // A workgroup per row and KV head finds the budget-th largest of its keys' ranks (32-bit numbers in the order of the weights, protected keys
-// above all): a histogram over the range that is left, 2048 bins, until a bin is one number -- at most three, mostly of L2 or LDS.  A
+// above all): a histogram over the range that is left, 2048 bins, until a bin stays whole -- at most three, one or two where the weights differ.  A
 // second launch moves keys and values: with the moves known it spreads over the chip.
 struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
 
@@ -813,33 +842,37 @@ __device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int rec
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// exclusive sums over the workgroup's 1024 threads of a and b; totals in ta, tb
-__device__ __forceinline__ void block_scan(int& a, int& b, int& ta, int& tb, int2* sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int ia = a, ib = b;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int ua = __shfl_up(ia, o, 64), ub = __shfl_up(ib, o, 64);
-    if (lane >= o) { ia += ua; ib += ub; }
-  }
-  if (lane == 63) sh[wave] = make_int2(ia, ib);
+// Across a wave in the vector unit (data-parallel primitives: a shift inside a row of 16, the last lane of a row to the next ones); a shuffle goes through
+// LDS, 120 cycles a step.  The last lane holds the whole.
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, int none, F&& f) {
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));      // row_shr:1
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));      // row_bcast:15 into rows 1 and 3
+  return f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));   // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ int wave_scan_sum(int v) { return wave_scan(v, 0, [](int a, int b) { return a + b; }); }
+
+// exclusive sum of v over the workgroup's threads, the sum of all in total
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, incl = wave_scan_sum(v);
+  if (lane == 63) sh[wave] = incl;
   __syncthreads();
-  int pa = 0, pb = 0;
-  ta = 0; tb = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    const int2 v = sh[w];
-    if (w < wave) { pa += v.x; pb += v.y; }
-    ta += v.x; tb += v.y;
-  }
+  const int w = wave_scan_sum(lane < THREADS / 64 ? sh[lane] : 0);
   __syncthreads();
-  a = pa + ia - a;
-  b = pb + ib - b;
+  total = __builtin_amdgcn_readlane(w, THREADS / 64 - 1);
+  const int u = __builtin_amdgcn_readfirstlane(wave);
+  return (u > 0 ? __builtin_amdgcn_readlane(w, u - 1) : 0) + incl - v;
 }
 
+// IN_LDS: the ranks stay on chip, slot i at i + i / 32 (a thread's slots lie side by side, threads' on different banks), otherwise they are made again from
+// weights and positions each time
 template <bool IN_LDS>
 __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, EvictWs ws) {
-  constexpr int BINS = 2048;
+  constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS;
   const int r = blockIdx.y, kh = blockIdx.x, n = held_keys(c, r);
   const size_t rk = (size_t)r * c.Hkv + kh;
   if (n <= budget) {
@@ -851,108 +884,125 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   const int recent_from = (int)max((int64_t)c.next[r] - keep_last, (int64_t)INT32_MIN);
   extern __shared__ uint32_t ranks[];
   __shared__ uint32_t hist[BINS];
-  __shared__ int2 scan[16];
-  __shared__ uint32_t sh_lo, sh_hi;
-  __shared__ int sh_prot, sh_bin, sh_above;
+  __shared__ int scan[16];
+  __shared__ uint32_t sh_lo[16], sh_hi[16];
+  __shared__ int sh_prot[16], sh_bin, sh_above, sh_in;
   bool crowded = false;
-  auto rank = [&](int i) { return IN_LDS ? ranks[i] : rank_of(wp[i], pp[i], keep_first, recent_from, crowded); };
+  auto rank = [&](int i) { return IN_LDS ? ranks[i + (i >> 5)] : rank_of(wp[i], pp[i], keep_first, recent_from, crowded); };
 
   // ranks, their range, and how many keys stay whatever their weight
+  uint32_t lo, hi;
+  int prot;
   for (int turn = 0; turn < 2; ++turn) {
-    if (threadIdx.x == 0) { sh_lo = 0xffffffffu; sh_hi = 0; sh_prot = 0; }
-    __syncthreads();
-    uint32_t lo = 0xffffffffu, hi = 0;
-    int prot = 0;
-    for (int i = threadIdx.x; i < n; i += 1024) {
+    lo = 0xffffffffu; hi = 0; prot = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
       const uint32_t k = rank_of(wp[i], pp[i], keep_first, recent_from, crowded);
-      if (IN_LDS) ranks[i] = k;
+      if (IN_LDS) ranks[i + (i >> 5)] = k;
       if (k == RANK_STAYS) ++prot;
       else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
-      prot += __shfl_xor(prot, o, 64);
-    }
-    if ((threadIdx.x & 63) == 0) { atomicMin(&sh_lo, lo); atomicMax(&sh_hi, hi); atomicAdd(&sh_prot, prot); }
+    for (int i = 0; i < PER; ++i) hist[threadIdx.x + i * THREADS] = 0;
+    lo = (uint32_t)wave_scan((int)lo, -1, [](int a, int b) { return (int)min((uint32_t)a, (uint32_t)b); });
+    hi = (uint32_t)wave_scan((int)hi, 0, [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); });
+    prot = wave_scan_sum(prot);
+    if ((threadIdx.x & 63) == 63) { sh_lo[threadIdx.x >> 6] = lo; sh_hi[threadIdx.x >> 6] = hi; sh_prot[threadIdx.x >> 6] = prot; }
     __syncthreads();
-    if (sh_prot <= budget) break;
+    lo = sh_lo[0]; hi = sh_hi[0]; prot = sh_prot[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) { lo = min(lo, sh_lo[w]); hi = max(hi, sh_hi[w]); prot += sh_prot[w]; }
+    if (prot <= budget) break;
     crowded = true;
     __syncthreads();
   }
-  // the number `cut` of which some stay: all above it do, of its own the `need` lowest slots
-  uint32_t cut = RANK_STAYS;
-  int need = budget;
-  if (sh_prot < budget) {
-    uint32_t lo = sh_lo, hi = sh_hi;
-    need = budget - sh_prot;
-    while (lo != hi) {                                             // the range shrinks by a factor of 1024 at least
-      const int shift = max(0, 21 - __clz(hi - lo));
-      for (int i = threadIdx.x; i < BINS; i += 1024) hist[i] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += 1024) {
+  // all ranks above `cut` stay, of those equal to it the `need` lowest slots
+  uint32_t cut = RANK_STAYS - 1;
+  int need = 0;
+  if (prot < budget) {
+    need = budget - prot;
+    for (;;) {                                                     // the range [lo, hi] holds the rank; it shrinks by a factor of 1024 at least
+      const int shift = max(0, 21 - __clz(hi - lo | 1u));
+      for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint32_t k = rank(i);
         if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
       }
       __syncthreads();
-      // bins from the highest down, two a thread
-      const int b1 = BINS - 1 - 2 * (int)threadIdx.x, h1 = (int)hist[b1], h0 = (int)hist[b1 - 1];
-      int before = h1 + h0, dummy = 0, t0, t1;
-      block_scan(before, dummy, t0, t1, scan);
-      if (before < need && before + h1 >= need) { sh_bin = b1; sh_above = before; }
-      else if (before + h1 < need && before + h1 + h0 >= need) { sh_bin = b1 - 1; sh_above = before + h1; }
+      // bins from the highest down, PER a thread
+      int h[PER], sum = 0, all;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = BINS - 1 - PER * (int)threadIdx.x - i;
+        h[i] = (int)hist[b];
+        hist[b] = 0;
+        sum += h[i];
+      }
+      sum = block_scan<THREADS>(sum, all, scan);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (sum < need && sum + h[i] >= need) { sh_bin = BINS - 1 - PER * (int)threadIdx.x - i; sh_above = sum; sh_in = h[i]; }
+        sum += h[i];
+      }
       __syncthreads();
       need -= sh_above;
       lo += (uint32_t)sh_bin << shift;
+      if (sh_in == need) {                                         // the whole bin stays
+        cut = lo - 1;
+        need = 0;
+        break;
+      }
+      if (shift == 0) {
+        cut = lo;
+        break;
+      }
       hi = min(hi, lo + ((1u << shift) - 1u));
     }
-    cut = lo;
   }
   // in the order of slots, four a thread and turn: which stay, and the i-th hole in front of `budget` gets the i-th that stays behind it
   int2* moves = ws.moves + rk * ws.most;
   int equal0 = 0, holes0 = 0, movers0 = 0;
-  for (int base = 0; base < n; base += 4096) {
+  for (int base = 0; base < n; base += 4 * THREADS) {
     const int i0 = base + 4 * threadIdx.x;
     uint32_t k[4];
-    int equal = 0, none = 0, te, tn;
+    int equal = 0, all_equal = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       k[j] = i0 + j < n ? rank(i0 + j) : 0;
       if (i0 + j < n && k[j] == cut) ++equal;
     }
-    block_scan(equal, none, te, tn, scan);
-    int at = equal0 + equal, holes = 0, movers = 0, th, tm;
+    int at = equal0 + (need > 0 ? block_scan<THREADS>(equal, all_equal, scan) : 0), both = 0, all;
     bool stays[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       stays[j] = i0 + j < n && (k[j] > cut || (k[j] == cut && at < need));
       if (i0 + j < n && k[j] == cut) ++at;
-      if (i0 + j < budget && !stays[j]) ++holes;
-      if (i0 + j >= budget && stays[j]) ++movers;
+      if (i0 + j < budget && !stays[j]) both += 1 << 16;         // (at most 4096 of either in a turn)
+      if (i0 + j >= budget && stays[j]) both += 1;
     }
-    block_scan(holes, movers, th, tm, scan);
+    both = block_scan<THREADS>(both, all, scan);
+    int holes = holes0 + (both >> 16), movers = movers0 + (both & 0xffff);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (i0 + j < budget && !stays[j]) moves[holes0 + holes++].y = i0 + j;
-      if (i0 + j >= budget && stays[j]) moves[movers0 + movers++].x = i0 + j;
+      if (i0 + j < budget && !stays[j]) moves[holes++].y = i0 + j;
+      if (i0 + j >= budget && stays[j]) moves[movers++].x = i0 + j;
     }
-    equal0 += te; holes0 += th; movers0 += tm;
+    equal0 += all_equal; holes0 += all >> 16; movers0 += all & 0xffff;
   }
-  __syncthreads();
   if (threadIdx.x == 0) ws.counts[rk] = movers0;
-  for (int i = threadIdx.x; i < movers0; i += 1024) {
-    const int2 m = moves[i];
-    wp[m.y] = wp[m.x];
-    pp[m.y] = pp[m.x];
-  }
 }
 
 __global__ __launch_bounds__(256) void evict_move_kernel(BoundedCache c, int budget, int row_pieces, EvictWs ws) {
   const int r = blockIdx.y / c.Hkv, kh = blockIdx.y % c.Hkv;
   if (blockIdx.x == 0 && kh == 0 && threadIdx.x == 0) c.len[r] = min(held_keys(c, r), budget);       // (nothing else of this launch reads it)
-  const int64_t total = (int64_t)ws.counts[blockIdx.y] * row_pieces;
+  const int count = ws.counts[blockIdx.y];
+  const int64_t total = (int64_t)count * row_pieces;
   const int2* moves = ws.moves + (size_t)blockIdx.y * ws.most;
+  float* w = c.weight + (size_t)blockIdx.y * c.cap;
+  int32_t* q = c.pos + (size_t)blockIdx.y * c.cap;
+  for (int e = blockIdx.x * 256 + threadIdx.x; e < count; e += gridDim.x * 256) {
+    const int2 m = moves[e];
+    w[m.y] = w[m.x];
+    q[m.y] = q[m.x];
+  }
   for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
     const int2 m = moves[e / row_pieces];
     const int p = (int)(e % row_pieces);
@@ -991,7 +1041,11 @@ int by_head(int D, F&& f) {                              // (mi_op_bounded_* hav
 
 int attend_splits(const BoundedCache& c, int Hq, int ncu) {
   const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16);
-  return std::max(1, std::min({MAX_SPLITS, (2 * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
+  // Short caches: one launch (321 keys, 8 KV heads: 8.7 us, in slices 10.8).  Otherwise four workgroups a CU, long caches two: 32 rows of up to 2048 keys 44.0 us with four,
+  // 47.4 with two, 46.8 with eight; 4 of 32761 keys 120, 117, 126.
+  if (c.cap <= 512) return 1;
+  const int wgs = c.cap >= 16384 ? 2 : 4;
+  return std::max(1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
 }
 // How a call is cut: units of nearly equal size, several times as many as the chip holds at once, so that its queues even them out.  First pass: 64 U queries by
 // `chunk` keys; second: 64 KS keys by `per` tiles of queries.
@@ -1038,7 +1092,8 @@ int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStre
   while ((16 << bits) < c.D) ++bits;
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
-    if (t.L == 1) {
+    // (steps of 32 rows: 4.3 us; 8 tokens of 8 rows: TODO)
+    if ((int64_t)t.L * (t.Hq + 2 * c.Hkv) << bits <= STEP_TASKS) {
       hipLaunchKernelGGL((append_kernel<T, true>), dim3(c.rows), dim3(1024), 0, st, c, t, bits);
     } else {
       const int64_t tasks = (int64_t)c.rows * t.L * (t.Hq + 2 * c.Hkv) << bits;
@@ -1098,8 +1153,9 @@ int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int 
   if (budget >= c.cap) return MI_OK;                     // no row can hold more
   const EvictWs w{(int32_t*)ws, (int2*)((char*)ws + up256((size_t)c.rows * c.Hkv * 4)), std::min(budget, c.cap - budget)};
   const dim3 grid(c.Hkv, c.rows);
-  if (c.cap <= 12288)                                    // ranks in LDS: 48 KiB
-    hipLaunchKernelGGL((evict_select_kernel<true>), grid, dim3(1024), (size_t)c.cap * 4, st, c, budget, keep_first, keep_last, w);
+  const size_t lds = ((size_t)c.cap + c.cap / 32 + 1) * 4;
+  if (c.cap <= 12288)                               // ranks in LDS: 50 KiB
+    hipLaunchKernelGGL((evict_select_kernel<true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, w);
   else
     hipLaunchKernelGGL((evict_select_kernel<false>), grid, dim3(1024), 0, st, c, budget, keep_first, keep_last, w);
   const int pieces = c.D * (int)dtype_size(c.dtype) / 16;
