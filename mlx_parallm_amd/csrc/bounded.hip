@@ -68,7 +68,8 @@ __device__ __forceinline__ Raw<NB> load_bits(const void* p) {
 template <typename T>
 struct alignas(16) Vec8 { T v[8]; };
 
-constexpr int STEP_TASKS = 8192;
+// (us, one launch / two: 1 token a row 2.9 / -, 4 tokens of 1 row 4.0 / 4.8, of 256 rows 6.3 / 8.3; 8 tokens 6.1 / 4.8, 6.9 / 5.8 for 64 rows)
+constexpr int STEP_TASKS = 2048;
 
 template <typename T, bool STEP>
 __global__ __launch_bounds__(STEP ? 1024 : 256) void append_kernel(BoundedCache c, BoundedTokens t, int lane_bits) {
@@ -1092,7 +1093,6 @@ int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStre
   while ((16 << bits) < c.D) ++bits;
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
-    // (steps of 32 rows: 4.3 us; 8 tokens of 8 rows: TODO)
     if ((int64_t)t.L * (t.Hq + 2 * c.Hkv) << bits <= STEP_TASKS) {
       hipLaunchKernelGGL((append_kernel<T, true>), dim3(c.rows), dim3(1024), 0, st, c, t, bits);
     } else {
