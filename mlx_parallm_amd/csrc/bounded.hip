@@ -33,6 +33,19 @@ __device__ __forceinline__ int64_t row_of_16(const BoundedCache& c, int r, int h
   return (((int64_t)blk * c.Hkv + h) << c.bs_shift) + (key & ((1 << c.bs_shift) - 1));
 }
 
+// Across a wave in the vector unit (data-parallel primitives: a shift inside a row of 16, the last lane of a row to the next ones); a shuffle goes through
+// LDS, 120 cycles a step.  The last lane holds the whole.
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, int none, F&& f) {
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));      // row_shr:1
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));      // row_bcast:15 into rows 1 and 3
+  return f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));   // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ int wave_scan_sum(int v) { return wave_scan(v, 0, [](int a, int b) { return a + b; }); }
+
 // raw bits of NB bytes (2, or a multiple of 4)
 template <int NB>
 struct Raw { uint32_t w[(NB + 3) / 4]; };
@@ -375,12 +388,33 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
     for (int j = 0; j < HB; ++j) s[j] = *(const f32x4*)(sp + (size_t)min(h0 + j, G - 1) * ws.ld);
   };
   fetch(0);
-  __shared__ float sh_m[MAX_GROUP], sh_r[MAX_GROUP];
+  float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
+  float w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = wp[min(key + i, c.cap - 1)];
+  // the output: its elements spread over the row's workgroups
+  const int groups = max(1, (n + JOIN_KEYS - 1) / JOIN_KEYS);
   const float* st = ws.stats + (size_t)(r * c.Hkv + kh) * splits * G * 2;
+  const float* pp = ws.part + (size_t)(r * c.Hkv + kh) * splits * G * D;
+  float o[8], om[8];
+  auto fetch_out = [&](int e, int i0) {
+    const int ee = min(e, G * D - 1), h = ee / D;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const size_t i = (size_t)max(0, min(i0 + j, ns - 1)) * G;
+      o[j] = pp[i * D + ee];
+      om[j] = st[(i + h) * 2];
+    }
+  };
+  const int e0 = blockIdx.x * 256 + threadIdx.x;
+  fetch_out(e0, 0);
+  __shared__ float sh_m[MAX_GROUP], sh_r[MAX_GROUP];
   for (int h = threadIdx.x >> 6; h < G; h += 4) {       // a wave per head, a lane per slice
     const int i = threadIdx.x & 63;
-    const float2 v = ns > 0 ? *(const float2*)(st + ((size_t)min(i, ns - 1) * G + h) * 2) : make_float2(-1e30f, 0.f);
-    const float M = wave_max(v.x), L = wave_sum(i < ns ? v.y * __builtin_amdgcn_exp2f(v.x - M) : 0.f);
+    const float2 v = *(const float2*)(st + ((size_t)max(0, min(i, ns - 1)) * G + h) * 2);
+    const float M = __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(i < ns ? v.x : -1e30f), __float_as_int(-1e30f), [](int a, int b) {
+      return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }), 63));
+    const float L = wave_sum(i < ns ? v.y * __builtin_amdgcn_exp2f(v.x - M) : 0.f);
     if (i == 0) { sh_m[h] = M; sh_r[h] = L != 0.f ? 1.f / L : 0.f; }
   }
   __syncthreads();
@@ -395,27 +429,17 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[j][i], sc, -sh_m[h0 + j])), sh_r[h0 + j], x[i]);
     }
-    float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap + key;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (key + i < n) wp[i] += x[i];
+      if (key + i < n) wp[key + i] = w[i] + x[i];
   }
-  // the output: its elements spread over the row's workgroups
-  const int groups = max(1, (n + JOIN_KEYS - 1) / JOIN_KEYS);
-  const float* pp = ws.part + (size_t)(r * c.Hkv + kh) * splits * G * D;
-  for (int e = blockIdx.x * 256 + threadIdx.x; e < G * D; e += groups * 256) {
+  for (int e = e0; e < G * D; e += groups * 256) {
     const int h = e / D;
     float x = 0.f;
     for (int i0 = 0; i0 < ns; i0 += 8) {
-      float o[8], m[8];
+      if (e != e0 || i0 > 0) fetch_out(e, i0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const size_t i = (size_t)min(i0 + j, ns - 1) * G;
-        o[j] = pp[i * D + e];
-        m[j] = st[(i + h) * 2];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], __builtin_amdgcn_exp2f(m[j] - sh_m[h]), x) : x;
+      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], __builtin_amdgcn_exp2f(om[j] - sh_m[h]), x) : x;
     }
     ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
   }
@@ -480,13 +504,13 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-// What a workgroup of a pass takes: KV heads side by side (a head stays on one XCD where their number is a multiple of eight), then slices, then tiles, those with
-// the most work first, then rows.  Rows side by side, of unequal lengths, stopped the dispatch: workgroups go round the shader engines in order, so one engine
-// got every workgroup of the longest row and the others waited behind it (4 prompts of up to 2048 tokens: 472 of 1024 places taken for the first 60 us of 88).
+// What a workgroup of a pass takes: KV heads side by side (a head stays on one XCD where their number is a multiple of eight), then slices, then rows, then
+// tiles, those with the most work first.  Rows change places from tile to tile: workgroups go round the shader engines in order, and where the n-th is always
+// of the longest row, one engine gets all of those and the others wait behind it (4 prompts of up to 2048 tokens: 472 of 1024 places taken for the first 60 us of 88).
 struct WeighPlace { int r, kh, slice, tile; };
-__device__ __forceinline__ WeighPlace weigh_place(const BoundedCache& c, int slices, int tiles) {
-  const int x = blockIdx.x / c.Hkv, y = x / slices;
-  return {y / tiles, (int)(blockIdx.x % c.Hkv), x % slices, y % tiles};
+__device__ __forceinline__ WeighPlace weigh_place(const BoundedCache& c, int slices) {
+  const int x = blockIdx.x / c.Hkv, y = x / slices, tile = y / c.rows;
+  return {(y + tile) % c.rows, (int)(blockIdx.x % c.Hkv), x % slices, tile};
 }
 
 // Queries of a workgroup of the first pass: U tiles of 16 a wave.  16 bits: two (four: 102 us instead of 88 for the pass over 4 prompts of up to 2048 tokens, two waves a SIMD; one: 106);
@@ -500,7 +524,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
   using St = Stage<T, D, ROWS>;
   const int G = a.Hq / c.Hkv;
   const int qtiles = gridDim.x / (c.rows * c.Hkv * splits);
-  const WeighPlace at = weigh_place(c, splits, qtiles);
+  const WeighPlace at = weigh_place(c, splits);
   const int r = at.r, kh = at.kh, split = at.slice;
   const WeighRow w = weigh_row(c, a, r);
   const int rho0 = (qtiles - 1 - at.tile) * QUERIES, rhos = w.queries * G;       // (the queries that see most keys first)
@@ -704,7 +728,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_a
   constexpr int D = 16 * E, ROWS = tile_rows<T, D>();
   using St = Stage<T, D, ROWS>;
   const int G = a.Hq / c.Hkv;
-  const WeighPlace at = weigh_place(c, slices, gridDim.x / (c.rows * c.Hkv * slices));
+  const WeighPlace at = weigh_place(c, slices);
   const int r = at.r, kh = at.kh;
   const WeighRow w = weigh_row(c, a, r);
   const int j0 = at.tile * 64 * KS;
@@ -843,19 +867,6 @@ __device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int rec
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Across a wave in the vector unit (data-parallel primitives: a shift inside a row of 16, the last lane of a row to the next ones); a shuffle goes through
-// LDS, 120 cycles a step.  The last lane holds the whole.
-template <typename F>
-__device__ __forceinline__ int wave_scan(int v, int none, F&& f) {
-  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));      // row_shr:1
-  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
-  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
-  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
-  v = f(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));      // row_bcast:15 into rows 1 and 3
-  return f(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));   // row_bcast:31 into rows 2 and 3
-}
-__device__ __forceinline__ int wave_scan_sum(int v) { return wave_scan(v, 0, [](int a, int b) { return a + b; }); }
-
 // exclusive sum of v over the workgroup's threads, the sum of all in total
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
@@ -896,11 +907,20 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   int prot;
   for (int turn = 0; turn < 2; ++turn) {
     lo = 0xffffffffu; hi = 0; prot = 0;
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      const uint32_t k = rank_of(wp[i], pp[i], keep_first, recent_from, crowded);
-      if (IN_LDS) ranks[i + (i >> 5)] = k;
-      if (k == RANK_STAYS) ++prot;
-      else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * THREADS) {        // (the loads of eight slots on their way together)
+      float w[8];
+      int32_t p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { const int i = min(i0 + j * THREADS, n - 1); w[j] = wp[i]; p[j] = pp[i]; }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = i0 + j * THREADS;
+        if (i >= n) continue;
+        const uint32_t k = rank_of(w[j], p[j], keep_first, recent_from, crowded);
+        if (IN_LDS) ranks[i + (i >> 5)] = k;
+        if (k == RANK_STAYS) ++prot;
+        else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
+      }
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) hist[threadIdx.x + i * THREADS] = 0;
@@ -923,9 +943,13 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
     need = budget - prot;
     for (;;) {                                                     // the range [lo, hi] holds the rank; it shrinks by a factor of 1024 at least
       const int shift = max(0, 21 - __clz(hi - lo | 1u));
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        const uint32_t k = rank(i);
-        if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> shift], 1u);
+      for (int i0 = threadIdx.x; i0 < n; i0 += 4 * THREADS) {
+        uint32_t k[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = rank(min(i0 + j * THREADS, n - 1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j * THREADS < n && k[j] >= lo && k[j] <= hi) atomicAdd(&hist[(k[j] - lo) >> shift], 1u);
       }
       __syncthreads();
       // bins from the highest down, PER a thread
