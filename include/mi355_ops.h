@@ -191,7 +191,8 @@ typedef struct mi_op_bounded_tokens {
 int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_tokens* t, void* stream);
 
 /* Attention of one query per row and head, q and out [rows][Hq][D], over all keys that the row holds (its own, just appended, among them); the weight that
- * every key receives, summed over the query heads of its KV head, is added to `weight`.  A row with nothing to see, or with counts[row] <= 0, gives zeros.
+ * every key receives, summed over the query heads of its KV head, is added to `weight`.  A row with nothing to see (no keys, or scores of -inf
+ * alone), or with counts[row] <= 0, gives zeros.
  * Hq / Hkv <= 128, Hq <= 8192 (all of these calls), scale > 0.  ws_bytes: mi_op_bounded_attend_ws, which needs no pointer. */
 uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq);
 int mi_op_bounded_attend(const mi_op_bounded_cache* c, const void* q, int Hq, const int32_t* counts, float scale, void* out, void* ws, uint64_t ws_bytes, void* stream);

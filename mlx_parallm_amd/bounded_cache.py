@@ -14,7 +14,7 @@ keys per row and KV head, on the kernels of ``csrc/bounded.hip`` (``mi_op_bounde
         cache.evict(budget, keep_first=4, keep_last=32)
 
 Everything is enqueued on torch's current stream of the cache's device, nothing waits: the lengths stay on the device, and the calls can be
-captured into a HIP graph.  There is no CPU fallback.
+captured into a HIP graph.  There are no gradients and no CPU fallback.
 """
 from __future__ import annotations
 

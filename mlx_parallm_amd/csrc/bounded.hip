@@ -19,8 +19,13 @@ using prefill::u32x2;
 using prefill::u32x4;
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -3.402823466e38f;      // where a maximum starts: finite, so that its distance to -inf (a masked score) is no NaN
 constexpr int MAX_SPLITS = 64;          // slices of a row's keys
 constexpr int MAX_GROUP = 128;          // query heads per KV head
+
+// exp(scale * (s - m)) of products s and m <= s's maximum, sc = scale * log2 e.  The difference first: at its maximum a score of any size weighs one (scale * s - scale * m in
+// one fused operation leaves the rounding of scale * m, 2^5 where a score is 2^30).
+__device__ __forceinline__ float weight_of(float s, float m, float sc) { return __builtin_amdgcn_exp2f((s - m) * sc); }
 
 __device__ __forceinline__ int held_keys(const BoundedCache& c, int r) { return min(max(c.len[r], 0), c.cap); }
 
@@ -264,7 +269,8 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
   Raw<E * (int)sizeof(T)> v[4 * SUB];
   q.load((const T*)a.q + ((size_t)r * a.Hq + kh * G + h0 + ln) * D, qd, ln < heads);
   const float sc = a.scale * LOG2E;
-  float m = -1e30f, l = 0.f;
+  const float step = 8.f / sc;                          // 2^8
+  float m = LOWEST, l = 0.f;
   f32x4 o[E];
 #pragma unroll
   for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -301,12 +307,12 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
       }
       if (ln < heads && key < s1) *(f32x4*)(sc_out + key) = s;         // (`ld` reaches to the tile's end)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i] * sc); }
+      for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
     }
-    if (__any(top > m + 8.f)) {
+    if (__any(top > m + step)) {
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - now);
+      const float now = fmaxf(m, top), f = weight_of(m, now, sc);
       m = now; l *= f;
 #pragma unroll
       for (int j = 0; j < E; ++j) o[j] *= f;
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
 #pragma unroll
     for (int t = 0; t < SUB; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { p[t][i] = __builtin_amdgcn_exp2f(fmaf(p[t][i], sc, -m)); l += p[t][i]; }
+      for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
     if constexpr (sizeof(T) == 2) add_values<T, E>(v, p, o);
     else add_values<T, E, SUB>(v, p, o);
   }
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
     M = fmaxf(fmaxf(sh_m[0][h], sh_m[1][h]), fmaxf(sh_m[2][h], sh_m[3][h]));
     L = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) { f[w] = __builtin_amdgcn_exp2f(sh_m[w][h] - M); L = fmaf(sh_l[w][h], f[w], L); }
+    for (int w = 0; w < NW; ++w) { f[w] = weight_of(sh_m[w][h], M, sc); L = fmaf(sh_l[w][h], f[w], L); }
   };
   const size_t slice = ((size_t)(r * c.Hkv + kh) * splits + split) * G + h0;
   for (int e = threadIdx.x; e < heads * D; e += 256) {
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
   float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
   for (int key = threadIdx.x; key < n; key += 256) {
     float x = 0.f;
-    for (int h = 0; h < heads; ++h) x = fmaf(__builtin_amdgcn_exp2f(fmaf(sp[(size_t)h * ws.ld + key], sc, -sh_o[0][0][h])), sh_o[0][1][h], x);
+    for (int h = 0; h < heads; ++h) x = fmaf(weight_of(sp[(size_t)h * ws.ld + key], sh_o[0][0][h], sc), sh_o[0][1][h], x);
     wp[key] += x;
   }
 }
@@ -408,18 +414,18 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
   };
   const int e0 = blockIdx.x * 256 + threadIdx.x;
   fetch_out(e0, 0);
+  const float sc = a.scale * LOG2E;
   __shared__ float sh_m[MAX_GROUP], sh_r[MAX_GROUP];
   for (int h = threadIdx.x >> 6; h < G; h += 4) {       // a wave per head, a lane per slice
     const int i = threadIdx.x & 63;
     const float2 v = *(const float2*)(st + ((size_t)max(0, min(i, ns - 1)) * G + h) * 2);
-    const float M = __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(i < ns ? v.x : -1e30f), __float_as_int(-1e30f), [](int a, int b) {
+    const float M = __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(i < ns ? v.x : LOWEST), __float_as_int(LOWEST), [](int a, int b) {
       return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }), 63));
-    const float L = wave_sum(i < ns ? v.y * __builtin_amdgcn_exp2f(v.x - M) : 0.f);
+    const float L = wave_sum(i < ns ? v.y * weight_of(v.x, M, sc) : 0.f);
     if (i == 0) { sh_m[h] = M; sh_r[h] = L != 0.f ? 1.f / L : 0.f; }
   }
   __syncthreads();
   if (key < n) {
-    const float sc = a.scale * LOG2E;
     f32x4 x{0.f, 0.f, 0.f, 0.f};
     for (int h0 = 0; h0 < G; h0 += HB) {
       if (h0 > 0) fetch(h0);
@@ -427,7 +433,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
       for (int j = 0; j < HB; ++j)
         if (h0 + j < G)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[j][i], sc, -sh_m[h0 + j])), sh_r[h0 + j], x[i]);
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(weight_of(s[j][i], sh_m[h0 + j], sc), sh_r[h0 + j], x[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -439,7 +445,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
     for (int i0 = 0; i0 < ns; i0 += 8) {
       if (e != e0 || i0 > 0) fetch_out(e, i0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], __builtin_amdgcn_exp2f(om[j] - sh_m[h]), x) : x;
+      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], weight_of(om[j], sh_m[h], sc), x) : x;
     }
     ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
   }
@@ -550,7 +556,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
   const float sc = a.scale * LOG2E;
   float m[U], l[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) { m[u] = -1e30f; l[u] = 0.f; }
+  for (int u = 0; u < U; ++u) { m[u] = LOWEST; l[u] = 0.f; }
   St st;
   // Not paged: a tile lies in one piece, behind one address.  Paged: the blocks of the tile after the next one are looked up in time.
   int block[St::N];
@@ -649,12 +655,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i]);
-          top = fmaxf(m[u], top * sc);
-          float x = l[u] * __builtin_amdgcn_exp2f(m[u] - top), y = 0.f;
+          top = fmaxf(m[u], top);
+          float x = l[u] * weight_of(m[u], top, sc), y = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x += __builtin_amdgcn_exp2f(fmaf(s[0][u][i], sc, -top));
-            y += __builtin_amdgcn_exp2f(fmaf(s[1][u][i], sc, -top));
+            x += weight_of(s[0][u][i], top, sc);
+            y += weight_of(s[1][u][i], top, sc);
           }
           m[u] = top; l[u] = x + y;
         }
@@ -671,7 +677,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1) {
       const float mo = __shfl_xor(m[u], off, 64), lo = __shfl_xor(l[u], off, 64), M = fmaxf(m[u], mo);
-      l[u] = l[u] * __builtin_amdgcn_exp2f(m[u] - M) + lo * __builtin_amdgcn_exp2f(mo - M);
+      l[u] = l[u] * weight_of(m[u], M, sc) + lo * weight_of(mo, M, sc);
       m[u] = M;
     }
     const int rho = rho0 + (wave * U + u) * 16 + ln;
@@ -695,7 +701,8 @@ __global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, Bounde
   if (rho >= w.queries * G) return;
   const size_t R = (size_t)a.L * G, rk = blockIdx.y;
   const int have = max(1, (weigh_most(w, G, rho / queries * queries, queries) + chunk - 1) / chunk);       // slices with keys that the query's workgroups saw
-  float M = -1e30f, L = 0.f;
+  const float sc = a.scale * LOG2E;
+  float M = LOWEST, L = 0.f;
   for (int i0 = 0; i0 < have; i0 += 8) {               // (eight loads on their way together)
     float2 p[8];
 #pragma unroll
@@ -703,10 +710,10 @@ __global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, Bounde
     float top = M;
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = fmaxf(top, p[j].x);
-    L *= __builtin_amdgcn_exp2f(M - top);
+    L *= weight_of(M, top, sc);
     M = top;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) L = i0 + j < have ? fmaf(p[j].y, __builtin_amdgcn_exp2f(p[j].x - M), L) : L;
+    for (int j = 0; j < 8; ++j) L = i0 + j < have ? fmaf(p[j].y, weight_of(p[j].x, M, sc), L) : L;
   }
   ws.stats[(rk * R + rho) * 2] = L != 0.f ? M : 0.f;
   ws.stats[(rk * R + rho) * 2 + 1] = L != 0.f ? 1.f / L : 0.f;
@@ -775,7 +782,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_a
 #pragma unroll
       for (int s = 0; s < St::N; ++s) st.w[s] = *(const u32x4*)(from + min((int64_t)St::row(s), (int64_t)left - 1) * ld_q * sizeof(T) + St::piece(s));
       sv = *(const float2*)(stat + min((int)threadIdx.x % ROWS, left - 1) * G * 2);
-      if ((int)threadIdx.x >= left) sv = make_float2(1e30f, 0.f);
+      if ((int)threadIdx.x >= left) sv = make_float2(INFINITY, 0.f);
     }
   };
   int g = t0 / wt.per_head, it = t0 % wt.per_head;
@@ -809,7 +816,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_a
         for (int t = 0; t < KS; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float p = __builtin_amdgcn_exp2f(fmaf(sv2[u & 1][t][i], sc, -ml.x));
+            float p = weight_of(sv2[u & 1][t][i], ml.x, sc);
             if (decltype(edge)::value && my0 + 16 * t + 4 * qd + i >= sees0 + u * 16 + ln) p = 0.f;
             x[t][i] = fmaf(p, ml.y, x[t][i]);
           }

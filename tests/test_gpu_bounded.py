@@ -252,6 +252,26 @@ def test_attend_infinite_keys(n):
     torch.testing.assert_close(out[0].double(), want[0], rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("n", [40, 1500])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_near_the_ends_of_the_type(n, sign):
+    """Scores of 1e33 and more, all above or all below zero: one key takes all the weight, of a token and of a prompt (whose last query repeats itself behind the end)."""
+    s = Setup(33, 1, 1, 64, n, [n], "float32")
+    c = s.cache
+    c.keys[0, 0] = sign * 1e16 * (1 + torch.arange(n, device="cuda").float())[:, None]
+    top = n - 1 if sign > 0 else 0
+    c.weights.zero_()
+    out = c.attend(torch.full((1, 2, 64), 1e17, device="cuda"))
+    assert torch.equal(out, c.values[0, 0, top].expand(1, 2, 64))
+    assert c.weights[0, 0, top] == 2 and c.weights.sum() == 2
+    c.weights.zero_()
+    c.weigh(torch.full((1, 3, 2, 64), 1e17, device="cuda"))
+    want = torch.zeros(n, device="cuda")
+    for i in range(3):
+        want[n - 3 + i if sign > 0 else 0] += 2
+    assert torch.equal(c.weights[0, 0], want)
+
+
 def test_attend_beyond_32_bits():
     """Element numbers of the second row's keys pass 2^31."""
     from mlx_parallm_amd.bounded_cache import BoundedKVCache
