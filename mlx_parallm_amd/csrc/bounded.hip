@@ -891,7 +891,7 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
 // weights and positions each time
 template <bool IN_LDS>
 __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, EvictWs ws) {
-  constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS;
+  constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS, FEW = 4;
   const int r = blockIdx.y, kh = blockIdx.x, n = held_keys(c, r);
   const size_t rk = (size_t)r * c.Hkv + kh;
   if (n <= budget) {
@@ -946,7 +946,18 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   // all ranks above `cut` stay, of those equal to it the `need` lowest slots
   uint32_t cut = RANK_STAYS - 1;
   int need = 0;
-  if (prot < budget) {
+  bool found = false;
+  if (n - budget <= FEW && !crowded) {                             // few leave: the least weighted alone (always, where it is one key a step)
+    int equal = 0, all;
+    for (int i = threadIdx.x; i < n; i += THREADS) equal += rank(i) == lo;
+    block_scan<THREADS>(equal, all, scan);
+    if (n - all <= budget) {
+      cut = lo;
+      need = budget - (n - all);
+      found = true;
+    }
+  }
+  if (prot < budget && !found) {
     need = budget - prot;
     for (;;) {                                                     // the range [lo, hi] holds the rank; it shrinks by a factor of 1024 at least
       const int shift = max(0, 21 - __clz(hi - lo | 1u));
