@@ -252,125 +252,133 @@ template <typename T, int E>
 __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
   constexpr int D = 16 * E, NW = 4;
   constexpr int SUB = sizeof(T) == 4 && E > 8 ? 1 : 2, KT = 16 * SUB;      // (float32 heads of 192 and 256: registers for 16 keys)
-  const int G = a.Hq / c.Hkv, split = blockIdx.x, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv, h0 = blockIdx.z * 16;
+  const int G = a.Hq / c.Hkv, split = blockIdx.x, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
-  const int heads = min(16, G - h0);
-  const bool alone = splits == 1 && gridDim.z == 1;     // nothing to join: this workgroup writes the results
+  const bool alone = splits == 1;                       // nothing to join: this workgroup takes all heads and writes the results
   const bool idle = a.counts != nullptr && a.counts[r] <= 0;
   const int n = idle ? 0 : held_keys(c, r);
   const int chunk = slice_keys(n, splits), s0 = split * chunk, s1 = min(n, s0 + chunk);
-  T* out = (T*)a.out + ((size_t)r * a.Hq + kh * G + h0) * D;
-  if (s0 >= s1 && !(alone && split == 0)) return;       // (the joining launch knows which slices there are)
+  if (s0 >= s1 && !alone) return;                       // (the joining launch knows which slices there are)
 
   __shared__ float sh_m[NW][16], sh_l[NW][16];
   __shared__ float sh_o[NW][16][D + 4];                 // (+ 4: the four quarters of a wave on different banks)
-
-  Frag<T, D> q, k[SUB];
-  Raw<E * (int)sizeof(T)> v[4 * SUB];
-  q.load((const T*)a.q + ((size_t)r * a.Hq + kh * G + h0 + ln) * D, qd, ln < heads);
+  __shared__ float all_m[MAX_GROUP], all_r[MAX_GROUP];
   const float sc = a.scale * LOG2E;
   const float step = 8.f / sc;                          // 2^8
-  float m = LOWEST, l = 0.f;
-  f32x4 o[E];
+  for (int h0 = blockIdx.z * 16; h0 < G; h0 += 16 * gridDim.z) {
+    const int heads = min(16, G - h0);
+    T* out = (T*)a.out + ((size_t)r * a.Hq + kh * G + h0) * D;
+    Frag<T, D> q, k[SUB];
+    Raw<E * (int)sizeof(T)> v[4 * SUB];
+    q.load((const T*)a.q + ((size_t)r * a.Hq + kh * G + h0 + ln) * D, qd, ln < heads);
+    float m = LOWEST, l = 0.f;
+    f32x4 o[E];
 #pragma unroll
-  for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;
+    for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;
 
-  for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
-    bool there[SUB];
+    for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
+      bool there[SUB];
 #pragma unroll
-    for (int t = 0; t < SUB; ++t) {
-      const int key = __builtin_amdgcn_readfirstlane(base + 16 * t);
-      const int64_t at = key < s1 ? row_of_16(c, r, kh, key) : -1;
-      there[t] = at >= 0;
-      const int last = there[t] ? min(15, s1 - 1 - key) : 0;           // (a clamped address: its scores are masked, its values cleared)
-      const T* kp = (const T*)c.k + (there[t] ? at : 0) * D;
-      const T* vp = (const T*)c.v + (there[t] ? at : 0) * D;
-      k[t].load(kp + (int64_t)min(ln, last) * D, qd);
+      for (int t = 0; t < SUB; ++t) {
+        const int key = __builtin_amdgcn_readfirstlane(base + 16 * t);
+        const int64_t at = key < s1 ? row_of_16(c, r, kh, key) : -1;
+        there[t] = at >= 0;
+        const int last = there[t] ? min(15, s1 - 1 - key) : 0;           // (a clamped address: its scores are masked, its values cleared)
+        const T* kp = (const T*)c.k + (there[t] ? at : 0) * D;
+        const T* vp = (const T*)c.v + (there[t] ? at : 0) * D;
+        k[t].load(kp + (int64_t)min(ln, last) * D, qd);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * t + i] = load_bits<E * (int)sizeof(T)>(vp + (int64_t)min(4 * qd + i, last) * D + ln * E);
-    }
-    float p[SUB][4];
-    float top = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < SUB; ++t) {
-      f32x4 s = dot16(k[t], q);
-      const int key = base + 16 * t + 4 * qd;
-      if (base + KT > s1 || !there[t]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (key + i >= s1 || !there[t]) {
-            s[i] = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
-          }
+        for (int i = 0; i < 4; ++i) v[4 * t + i] = load_bits<E * (int)sizeof(T)>(vp + (int64_t)min(4 * qd + i, last) * D + ln * E);
       }
-      if (ln < heads && key < s1) *(f32x4*)(sc_out + key) = s;         // (`ld` reaches to the tile's end)
+      float p[SUB][4];
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
+      for (int t = 0; t < SUB; ++t) {
+        f32x4 s = dot16(k[t], q);
+        const int key = base + 16 * t + 4 * qd;
+        if (base + KT > s1 || !there[t]) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key + i >= s1 || !there[t]) {
+              s[i] = -INFINITY;
+#pragma unroll
+              for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
+            }
+        }
+        if (ln < heads && key < s1) *(f32x4*)(sc_out + key) = s;         // (`ld` reaches to the tile's end)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
+      }
+      if (__any(top > m + step)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float now = fmaxf(m, top), f = weight_of(m, now, sc);
+        m = now; l *= f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) o[j] *= f;
+      }
+#pragma unroll
+      for (int t = 0; t < SUB; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
+      if constexpr (sizeof(T) == 2) add_values<T, E>(v, p, o);
+      else add_values<T, E, SUB>(v, p, o);
     }
-    if (__any(top > m + step)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float now = fmaxf(m, top), f = weight_of(m, now, sc);
-      m = now; l *= f;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (lane < 16) { sh_m[wave][ln] = m; sh_l[wave][ln] = l; }
+    if (ln < heads) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) o[j] *= f;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < E; ++j) sh_o[wave][ln][(4 * qd + i) * E + j] = o[j][i];
     }
+    __syncthreads();
+    // the four waves' states
+    auto join = [&](int h, float& M, float& L, float (&f)[NW]) {
+      M = fmaxf(fmaxf(sh_m[0][h], sh_m[1][h]), fmaxf(sh_m[2][h], sh_m[3][h]));
+      L = 0.f;
 #pragma unroll
-    for (int t = 0; t < SUB; ++t)
+      for (int w = 0; w < NW; ++w) { f[w] = weight_of(sh_m[w][h], M, sc); L = fmaf(sh_l[w][h], f[w], L); }
+    };
+    const size_t slice = ((size_t)(r * c.Hkv + kh) * splits + split) * G + h0;
+    for (int e = threadIdx.x; e < heads * D; e += 256) {
+      const int h = e / D, d = e % D;
+      float M, L, f[NW], x = 0.f;
+      join(h, M, L, f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
-    if constexpr (sizeof(T) == 2) add_values<T, E>(v, p, o);
-    else add_values<T, E, SUB>(v, p, o);
-  }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (lane < 16) { sh_m[wave][ln] = m; sh_l[wave][ln] = l; }
-  if (ln < heads) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < E; ++j) sh_o[wave][ln][(4 * qd + i) * E + j] = o[j][i];
-  }
-  __syncthreads();
-  // the four waves' states
-  auto join = [&](int h, float& M, float& L, float (&f)[NW]) {
-    M = fmaxf(fmaxf(sh_m[0][h], sh_m[1][h]), fmaxf(sh_m[2][h], sh_m[3][h]));
-    L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) { f[w] = weight_of(sh_m[w][h], M, sc); L = fmaf(sh_l[w][h], f[w], L); }
-  };
-  const size_t slice = ((size_t)(r * c.Hkv + kh) * splits + split) * G + h0;
-  for (int e = threadIdx.x; e < heads * D; e += 256) {
-    const int h = e / D, d = e % D;
-    float M, L, f[NW], x = 0.f;
-    join(h, M, L, f);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) x = fmaf(sh_o[w][h][d], f[w], x);
-    if (alone) {
-      out[e] = (T)(L != 0.f ? x / L : 0.f);
-    } else {
-      ws.part[slice * D + e] = x;
-      if (d == 0) { ws.stats[(slice + h) * 2] = M; ws.stats[(slice + h) * 2 + 1] = L; }
+      for (int w = 0; w < NW; ++w) x = fmaf(sh_o[w][h][d], f[w], x);
+      if (alone) {
+        out[e] = (T)(L != 0.f ? x / L : 0.f);
+      } else {
+        ws.part[slice * D + e] = x;
+        if (d == 0) { ws.stats[(slice + h) * 2] = M; ws.stats[(slice + h) * 2 + 1] = L; }
+      }
     }
+    if (!alone) return;
+    if (threadIdx.x < heads) {
+      float M, L, f[NW];
+      join(threadIdx.x, M, L, f);
+      all_m[h0 + threadIdx.x] = M;
+      all_r[h0 + threadIdx.x] = L != 0.f ? 1.f / L : 0.f;
+    }
+    __syncthreads();
   }
-  if (!alone || n == 0) return;
   // what every key received: its scores lie in the workspace, written by this workgroup in front of the barrier above
-  __syncthreads();
-  if (threadIdx.x < heads) {
-    float M, L, f[NW];
-    join(threadIdx.x, M, L, f);
-    sh_o[0][0][threadIdx.x] = M;
-    sh_o[0][1][threadIdx.x] = L != 0.f ? 1.f / L : 0.f;
-  }
-  __syncthreads();
   const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld;
   float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
   for (int key = threadIdx.x; key < n; key += 256) {
+    const float w = wp[key];
     float x = 0.f;
-    for (int h = 0; h < heads; ++h) x = fmaf(weight_of(sp[(size_t)h * ws.ld + key], sh_o[0][0][h], sc), sh_o[0][1][h], x);
-    wp[key] += x;
+    for (int h0 = 0; h0 < G; h0 += 8) {
+      float s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = sp[(size_t)min(h0 + j, G - 1) * ws.ld + key];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x = h0 + j < G ? fmaf(weight_of(s[j], all_m[h0 + j], sc), all_r[h0 + j], x) : x;
+    }
+    wp[key] = w + x;
   }
 }
 
@@ -1082,13 +1090,14 @@ int by_head(int D, F&& f) {                              // (mi_op_bounded_* hav
   return fail(MI_ERR_UNSUPPORTED, "bounded cache: head_dim");
 }
 
+// Slices of a row's keys; one: the kernel needs no joining launch, and its workgroups take all query heads of a KV head, 16 at a time.  That is for short caches: 321 keys of 8 KV
+// heads 8.7 us, in slices 10.8.  Otherwise four workgroups a CU, for long caches two: 32 rows of up to 2048 keys 44.0 us with four, 47.4 with two, 46.8 with eight; 4 of 32761 keys
+// 120, 117, 126.
 int attend_splits(const BoundedCache& c, int Hq, int ncu) {
-  const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16);
-  // Short caches: one launch (321 keys, 8 KV heads: 8.7 us, in slices 10.8).  Otherwise four workgroups a CU, long caches two: 32 rows of up to 2048 keys 44.0 us with four,
-  // 47.4 with two, 46.8 with eight; 4 of 32761 keys 120, 117, 126.
-  if (c.cap <= 512) return 1;
+  const int groups = (Hq / c.Hkv + 15) / 16, tiles = c.rows * c.Hkv * groups;
+  if (c.cap <= 512 && c.cap * groups <= 1024) return 1;
   const int wgs = c.cap >= 16384 ? 2 : 4;
-  return std::max(1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
+  return std::max(groups > 1 ? 2 : 1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
 }
 // How a call is cut: units of nearly equal size, several times as many as the chip holds at once, so that its queues even them out.  First pass: 64 U queries by
 // `chunk` keys; second: 64 KS keys by `per` tiles of queries.
@@ -1103,7 +1112,7 @@ WeighPlan weigh_plan(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   auto key_tiles = [&](int ks) { return pairs * ((c.cap + 64 * ks - 1) / (64 * ks)); };
   p.ks = !f32 && key_tiles(2) >= ncu ? 2 : 1;
   const int rows = c.D * (int)dtype_size(c.dtype) <= 256 ? 64 : 32;
-  const int64_t tiles = (int64_t)G * ((L + rows - 1) / rows), least = f32 ? 4 : 8;
+  const int64_t tiles = (int64_t)G * ((L + rows - 1) / rows), least = f32 ? 2 : 8;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({MAX_SPLITS, 24 * ncu / key_tiles(p.ks), (tiles + least - 1) / least}));
   p.per = (int)((tiles + want - 1) / want);
   p.slices = (int)((tiles + p.per - 1) / p.per);
@@ -1157,9 +1166,9 @@ int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* w
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
     return by_head(c.D, [&](auto e) {
-      const dim3 grid(splits, c.rows * c.Hkv, (G + 15) / 16);
+      const dim3 grid(splits, c.rows * c.Hkv, splits > 1 ? (G + 15) / 16 : 1);
       hipLaunchKernelGGL((attend_kernel<T, decltype(e)::value>), grid, dim3(256), 0, st, c, a, w, splits);
-      if (splits > 1 || G > 16)
+      if (splits > 1)
         hipLaunchKernelGGL((attend_join_kernel<T>), dim3((c.cap + JOIN_KEYS - 1) / JOIN_KEYS, c.rows * c.Hkv), dim3(256), 0, st, c, a, w, splits);
       MI_HIP(hipGetLastError());
       return MI_OK;
