@@ -163,7 +163,8 @@ int mi_op_sample(float* logits, int B, int V, float temperature, float top_p, co
  * Calls on one cache follow one another in the order of its stream; ws is the call's own until it has run.  All pointers are device memory,
  * arrays are contiguous and aligned to 16 bytes.  What lies in `len`, `next`, `counts` and the block table is read on the device and cannot be refused: a
  * length outside [0, cap] counts as the nearer end, a table entry outside [0, n_blocks) names no block: its keys take no part in attention, and nothing is
- * written for them.  Slots behind a row's length keep what they hold. */
+ * written for them.  Slots behind a row's length keep what they hold.  The attention of a prompt itself: mi_op_attention_prefill on the same arrays, its
+ * offsets the lengths in front of the append. */
 typedef struct mi_op_bounded_cache {
   int32_t rows, Hkv, D, dtype;       /* D: 16, 32, 64, 96, 128, 192, 256; dtype MI_F32 / MI_BF16 / MI_F16: of K, V, queries, outputs and norm weights */
   int32_t cap;                       /* slots per row (paged: at most bt_stride blocks) */

@@ -5,7 +5,7 @@ keys per row and KV head, on the kernels of ``csrc/bounded.hip`` (``mi_op_bounde
 
     cache = BoundedKVCache.create(rows, kv_heads, head_dim, capacity, dtype="bfloat16")
     q = cache.append(qkv, heads, cos, sin, counts=prompt_lengths)      # norms, rotation, append; [rows, L, heads, head_dim]
-    ...                                                                # the prompt's attention
+    ...                                                                # the prompt's attention (mi_op_attention_prefill reads the same arrays)
     cache.weigh(q, counts=prompt_lengths)                              # what weight the prompt's queries give every key
     cache.evict(budget, keep_first=4, keep_last=32)
     while generating:

@@ -82,7 +82,9 @@ __device__ __forceinline__ Raw<NB> load_bits(const void* p) {
 // One lane takes 8 + 8 elements of a head, i .. i + 8 and i + D / 2 .. i + D / 2 + 8 (the two halves of a rotation's pairs), a power of two of
 // lanes a head.  All in 32 bits, rounded once, to what is stored.
 // STEP (few tokens a row): a workgroup per row, which moves the row's length and next position itself.  Otherwise the tasks of all tokens lie
-// side by side and a second launch moves them.
+// side by side and a second launch moves them (its atomics would come to one address from 1536 workgroups).
+// Bound by memory: 8 x 1024 float32 tokens of 48 heads of 128, 407 MB, 74 us (5.5 TB/s; a copy of 4 GiB: 4.65 read and written) + 5 for the second launch; a step by its launch and one round
+// trip: 2.4 us for one row, 4.2 for 32.
 template <typename T>
 struct alignas(16) Vec8 { T v[8]; };
 
@@ -172,6 +174,10 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // it.  A lane loads E = D / 16 elements of 8 keys' values -- whole rows across 16 lanes -- and transposes its 8 x E block in registers
 // (v_perm); column n of output tile j is element n E + j.  P goes in as two 16-bit terms (2^-17).  float32: 16 x 16 x 4 products, no
 // transposition.  The largest score so far is taken in when a new one exceeds it by 2^8, not at every tile.
+// What a key weighs needs the final maximum and sum of every head, so the products are kept (4 bytes a head and key, 3 % of 16-bit keys and values at 4 heads) and read by whoever has
+// them: this workgroup where it is alone, else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
+// Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
+// launches' heads; 8 rows of 1025 float32 keys, 68 MB, 20.7 + 4.8: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
 // A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
 template <typename T, int D>
 struct Frag {
@@ -464,6 +470,9 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 // over S^T = K Q^T: the largest score and the sum of every query (a lane keeps its own over the keys that it holds; four lanes join at the
 // end), then the sum over the queries for every key.  The first keeps queries in registers and passes keys through LDS, the second the
 // other way round.
+// Bound by the matrix cores and the exponentials beside them, which hardly overlap: a block of 64 scores costs 16 cycles of the one and 15 to 20 of the other at D = 128.  4 prompts of 819 to 2048 bf16
+// tokens, 32 / 8 heads: 64 + 71 + 5 us, 2 x 37 GFLOP, 560 TFLOP/s over both passes (a product of 8192 x 8192 x 8192: 1135; the clock under this load is 1.95 GHz).  2 prompts of 700 float32 tokens 58 + 5
+// + 56 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
 // Workspace: [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
 // queries, [slice][row][KV head][ld] sums.
 struct WeighWs { float* stats; float* parts; float* sums; int ld; };
@@ -871,6 +880,8 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 // A workgroup per row and KV head finds the budget-th largest of its keys' ranks (32-bit numbers in the order of the weights, protected keys
 // above all): a histogram over the range that is left, 2048 bins, until a bin stays whole -- at most three, one or two where the weights differ.  A
 // second launch moves keys and values: with the moves known it spreads over the chip.
+// 64 rows and heads of 8192 keys down to 1024: 12.8 us (a chain of barriers on 64 CUs; the first histogram's range is wasted on the gap between zero and the least weight) + 15 us to move 59 MB (3.9 TB/s in rows of
+// 256 bytes); 256 of 1025 down to 1024: 6.5 + 3.
 struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
 
 // Where more keys are protected than the budget holds, they alone are ranked (`crowded`).

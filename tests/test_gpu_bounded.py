@@ -463,6 +463,37 @@ def test_generation_in_a_bounded_cache(dtype, paged, norm):
     assert c.lengths.tolist() == [24, 24, 24] and c.next_positions.tolist() == [70, 33, 44]
 
 
+def test_the_frameworks_prompt_attention_reads_the_same_cache():
+    """The second part of a prompt behind an eviction: mi_op_attention_prefill on the cache's arrays, offsets = lengths in front of the append."""
+    import ctypes as C
+
+    from mlx_parallm_amd import _lib as lib
+    from tests.gpu_helpers import attn_shape, ptr
+
+    D, Hq, Hkv, R, L = 128, 8, 2, 2, 20
+    s = Setup(62, R, Hkv, D, 128, [60, 41], "bfloat16", True)
+    c, m = s.cache, s.model
+    evict_once(s, 40, 4, 8)
+    cos, sin = angles(200, D)
+    qkv = s.randn(R, L, (Hq + 2 * Hkv) * D)
+    before = c.lengths.clone()
+    q = c.append(qkv.cuda(), Hq, cos.cuda(), sin.cuda())
+    m.append(f64(qkv), Hq, cos.numpy(), sin.numpy())
+    m.k, m.v = s.caches()
+    out = torch.empty((R, L, Hq, D), dtype=torch.bfloat16, device="cuda")
+    shape = attn_shape(R, L, Hq, Hkv, D, "bfloat16", "bfloat16", 0, 128)
+    torch.cuda.synchronize()
+    lib.check(lib.lib().mi_op_attention_prefill(C.byref(shape), ptr(c.block_table), c.block_table.shape[1], 4, ptr(q), ptr(c.keys), ptr(c.values), ptr(before), ptr(out), D ** -0.5, 1, None, None))
+    for i in range(L):
+        sees = Model(m.k, m.v, before.cpu().numpy() + i + 1, m.next, m.pos, m.w)
+        want, tol, _ = sees.attend(f64(q[:, i]), D ** -0.5, "bfloat16")
+        within(f64(out[:, i]), want, tol + 2 ** -8 * np.abs(want) + 1e-3)      # (that kernel's own roundings; a wrong key would be off by its weight, 1 / 60)
+    c.weigh(q)
+    s.check_meta(m.weigh(f64(q), D ** -0.5))
+    m.w[:] = f64(c.weights)
+    evict_once(s, 40, 4, 8)
+
+
 def steps(c, qkvs, Hq, cos, sin):
     outs = []
     for x in qkvs:
