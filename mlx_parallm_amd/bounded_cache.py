@@ -82,7 +82,9 @@ class BoundedKVCache:
     @classmethod
     def create(cls, rows: int, kv_heads: int, head_dim: int, capacity: int, dtype="bfloat16", *, block_tokens: int = 0, device="cuda") -> "BoundedKVCache":
         """An empty cache of its own tensors.  block_tokens > 0: paged, every row with blocks of its own for `capacity` slots."""
-        dt = _NAMES[dtype] if isinstance(dtype, str) else dtype
+        dt = _NAMES.get(dtype) if isinstance(dtype, str) else dtype
+        if dt not in _DTYPES:
+            raise ValueError(f"dtype: {', '.join(_NAMES)}; got {dtype}")
         shape, table = (rows, kv_heads, capacity, head_dim), None
         if block_tokens:
             per_row = -(-capacity // block_tokens)

@@ -85,6 +85,7 @@ __device__ __forceinline__ Raw<NB> load_bits(const void* p) {
 // side by side and a second launch moves them (its atomics would come to one address from 1536 workgroups).
 // Bound by memory: 8 x 1024 float32 tokens of 48 heads of 128, 407 MB, 74 us (5.5 TB/s; a copy of 4 GiB: 4.65 read and written) + 5 for the second launch; a step by its launch and one round
 // trip: 2.4 us for one row, 4.2 for 32.
+
 template <typename T>
 struct alignas(16) Vec8 { T v[8]; };
 
@@ -178,6 +179,7 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // them: this workgroup where it is alone, else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
 // Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
 // launches' heads; 8 rows of 1025 float32 keys, 68 MB, 20.7 + 4.8: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
+
 // A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
 template <typename T, int D>
 struct Frag {

@@ -108,6 +108,12 @@ def test_tensors_that_are_no_cache(change, text):
         BoundedKVCache(**parts(**change))
 
 
+def test_create_refuses():
+    for kw in (dict(dtype="int8"), dict(dtype=torch.float64), dict(block_tokens=24), dict(block_tokens=8)):
+        with pytest.raises(ValueError):
+            BoundedKVCache.create(1, 1, 64, 50, **{"device": "cpu", **kw})
+
+
 def test_arguments_that_do_not_fit_the_cache():
     c = BoundedKVCache(**parts())
     b = dict(dtype=torch.bfloat16)
