@@ -173,6 +173,7 @@ typedef struct mi_op_bounded_cache {
   const int32_t* btab;               /* [rows][bt_stride], or NULL: not paged */
   int32_t* len; int32_t* next;       /* [rows] slots filled; position of the row's next token */
   int32_t* pos; float* weight;       /* [rows][Hkv][cap] position of the key in a slot; attention weight that it has received */
+  int32_t* tickets;                  /* [rows] zeros, which every call leaves as zeros */
 } mi_op_bounded_cache;
 
 /* New tokens: queries and keys are normed per head (x / sqrt(mean x^2 + eps) * w; no norm where the weights are NULL), rotated by the angles of their

@@ -99,7 +99,8 @@ class OpAttnShape(C.Structure):
 class OpBoundedCache(C.Structure):
     _fields_ = [("rows", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32), ("cap", C.c_int32),
                 ("n_blocks", C.c_int32), ("bt_stride", C.c_int32), ("bs_shift", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
-                ("btab", C.c_void_p), ("len", C.c_void_p), ("next", C.c_void_p), ("pos", C.c_void_p), ("weight", C.c_void_p)]
+                ("btab", C.c_void_p), ("len", C.c_void_p), ("next", C.c_void_p), ("pos", C.c_void_p), ("weight", C.c_void_p),
+                ("tickets", C.c_void_p)]
 
 
 class OpBoundedTokens(C.Structure):

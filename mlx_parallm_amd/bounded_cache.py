@@ -77,6 +77,9 @@ class BoundedKVCache:
             c.n_blocks, c.bt_stride, c.bs_shift = keys.shape[0], block_table.shape[1], tokens.bit_length() - 1
         c.k, c.v, c.btab = keys.data_ptr(), values.data_ptr(), _ptr(block_table)
         c.len, c.next, c.pos, c.weight = lengths.data_ptr(), next_positions.data_ptr(), positions.data_ptr(), weights.data_ptr()
+        # copied from the host, which waits: calls may come on any stream from here on (and a cache is not made while a graph is captured)
+        self._tickets = torch.zeros(rows, dtype=torch.int32).to(self.device)
+        c.tickets = self._tickets.data_ptr()
         self._c, self._ref, self._lib = c, C.byref(c), L.lib()
 
     @classmethod
@@ -133,7 +136,7 @@ class BoundedKVCache:
         out = torch.empty_like(q)
         n = self._lib.mi_op_bounded_attend_ws(self._ref, heads)
         ws = self._workspace(n)
-        self._call(self._lib.mi_op_bounded_attend, self._ref, q.data_ptr(), heads, self._counts(counts), self._scale(scale), out.data_ptr(), ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_attend, self._ref, q.data_ptr(), heads, self._counts(counts), self._scale(scale), out.data_ptr(), _ptr(ws), n)
         return out
 
     def weigh(self, q, scale: Optional[float] = None, *, counts=None, last: int = 0) -> None:
@@ -145,14 +148,14 @@ class BoundedKVCache:
         q = q.contiguous()
         n = self._lib.mi_op_bounded_weigh_ws(self._ref, q.shape[1], q.shape[2], last)
         ws = self._workspace(n)
-        self._call(self._lib.mi_op_bounded_weigh, self._ref, q.data_ptr(), q.shape[1], q.shape[2], self._counts(counts), last, self._scale(scale), ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_weigh, self._ref, q.data_ptr(), q.shape[1], q.shape[2], self._counts(counts), last, self._scale(scale), _ptr(ws), n)
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_last: int = 0) -> None:
         """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last`` before all
         others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it."""
         n = self._lib.mi_op_bounded_evict_ws(self._ref, budget)
         ws = self._workspace(n)
-        self._call(self._lib.mi_op_bounded_evict, self._ref, budget, keep_first, keep_last, ws.data_ptr(), n)
+        self._call(self._lib.mi_op_bounded_evict, self._ref, budget, keep_first, keep_last, _ptr(ws), n)
 
     def reset(self) -> None:
         """Every row empty, its next token at position 0."""
@@ -178,7 +181,7 @@ class BoundedKVCache:
 
     def _workspace(self, n: int):
         # of torch's allocator, call by call: its blocks go round in the order of the stream, and a captured graph has its own
-        return self.lengths.new_empty((n + 3) // 4)
+        return self.lengths.new_empty((n + 3) // 4) if n else None
 
     def _call(self, fn, *args) -> None:
         if self.device.type != "cuda":

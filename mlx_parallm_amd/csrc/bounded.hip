@@ -176,7 +176,7 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // (v_perm); column n of output tile j is element n E + j.  P goes in as two 16-bit terms (2^-17).  float32: 16 x 16 x 4 products, no
 // transposition.  The largest score so far is taken in when a new one exceeds it by 2^8, not at every tile.
 // What a key weighs needs the final maximum and sum of every head, so the products are kept (4 bytes a head and key, 3 % of 16-bit keys and values at 4 heads) and read by whoever has
-// them: this workgroup where it is alone, else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
+// them: the workgroup itself where it is alone (`ALONE`), else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
 // Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
 // launches' heads; 8 rows of 1025 float32 keys, 68 MB, 20.7 + 4.8: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
 
@@ -250,27 +250,30 @@ __device__ __forceinline__ void add_values(const Raw<E * 4> (&v)[4 * SUB], const
 // the slice of a row's keys that each of `splits` workgroups takes: a multiple of 128 (one tile of 32 for each of four waves)
 __device__ __forceinline__ int slice_keys(int n, int splits) { return ((n + splits - 1) / splits + 127) & ~127; }
 
-// Workspace of a call: scores [row][KV head][query head of the group][cap, in 32s] as products (no scale), then of every slice the largest score
+// Short caches: one workgroup takes all keys and query heads of a KV head (16 at a time) and keeps the scores in LDS.  Otherwise slices and a joining launch.
+constexpr int ALONE_SCORES = 7168;                     // keys (in 32s) times heads: 28 KiB
+
+// Workspace of a call in slices: scores [row][KV head][query head of the group][cap, in 32s] as products (no scale), then of every slice the largest score
 // and the sum [row][KV head][slice][head][2], then its output [row][KV head][slice][head][D].
 struct AttendWs {
   float* scores; float* stats; float* part; int ld;
 };
 
-template <typename T, int E>
+template <typename T, int E, bool ALONE>
 __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
   constexpr int D = 16 * E, NW = 4;
   constexpr int SUB = sizeof(T) == 4 && E > 8 ? 1 : 2, KT = 16 * SUB;      // (float32 heads of 192 and 256: registers for 16 keys)
   const int G = a.Hq / c.Hkv, split = blockIdx.x, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
-  const bool alone = splits == 1;                       // nothing to join: this workgroup takes all heads and writes the results
   const bool idle = a.counts != nullptr && a.counts[r] <= 0;
   const int n = idle ? 0 : held_keys(c, r);
   const int chunk = slice_keys(n, splits), s0 = split * chunk, s1 = min(n, s0 + chunk);
-  if (s0 >= s1 && !alone) return;                       // (the joining launch knows which slices there are)
+  if (!ALONE && s0 >= s1) return;                       // (the joining launch knows which slices there are)
 
   __shared__ float sh_m[NW][16], sh_l[NW][16];
   __shared__ float sh_o[NW][16][D + 4];                 // (+ 4: the four quarters of a wave on different banks)
-  __shared__ float all_m[MAX_GROUP], all_r[MAX_GROUP];
+  __shared__ float all_m[ALONE ? MAX_GROUP : 1], all_r[ALONE ? MAX_GROUP : 1];
+  __shared__ __align__(16) float all_s[ALONE ? ALONE_SCORES : 4];
   const float sc = a.scale * LOG2E;
   const float step = 8.f / sc;                          // 2^8
   for (int h0 = blockIdx.z * 16; h0 < G; h0 += 16 * gridDim.z) {
@@ -283,7 +286,8 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
     f32x4 o[E];
 #pragma unroll
     for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;
+    float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;      // (in slices)
+    const int sh_at = (h0 + ln) * ws.ld;                                                // (alone)
 
     for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
       bool there[SUB];
@@ -314,7 +318,10 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
               for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
             }
         }
-        if (ln < heads && key < s1) *(f32x4*)(sc_out + key) = s;         // (`ld` reaches to the tile's end)
+        if (ln < heads && key < s1) {                                    // (`ld` reaches to the tile's end)
+          if constexpr (ALONE) *(f32x4*)&all_s[sh_at + key] = s;
+          else *(f32x4*)(sc_out + key) = s;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
       }
@@ -357,36 +364,31 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
       join(h, M, L, f);
 #pragma unroll
       for (int w = 0; w < NW; ++w) x = fmaf(sh_o[w][h][d], f[w], x);
-      if (alone) {
+      if constexpr (ALONE) {
         out[e] = (T)(L != 0.f ? x / L : 0.f);
       } else {
         ws.part[slice * D + e] = x;
         if (d == 0) { ws.stats[(slice + h) * 2] = M; ws.stats[(slice + h) * 2 + 1] = L; }
       }
     }
-    if (!alone) return;
-    if (threadIdx.x < heads) {
-      float M, L, f[NW];
-      join(threadIdx.x, M, L, f);
-      all_m[h0 + threadIdx.x] = M;
-      all_r[h0 + threadIdx.x] = L != 0.f ? 1.f / L : 0.f;
+    if constexpr (ALONE) {
+      if (threadIdx.x < heads) {
+        float M, L, f[NW];
+        join(threadIdx.x, M, L, f);
+        all_m[h0 + threadIdx.x] = M;
+        all_r[h0 + threadIdx.x] = L != 0.f ? 1.f / L : 0.f;
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
-  // what every key received: its scores lie in the workspace, written by this workgroup in front of the barrier above
-  const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld;
-  float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
-  for (int key = threadIdx.x; key < n; key += 256) {
-    const float w = wp[key];
-    float x = 0.f;
-    for (int h0 = 0; h0 < G; h0 += 8) {
-      float s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = sp[(size_t)min(h0 + j, G - 1) * ws.ld + key];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x = h0 + j < G ? fmaf(weight_of(s[j], all_m[h0 + j], sc), all_r[h0 + j], x) : x;
+  if constexpr (ALONE) {                                // what every key received
+    float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap;
+    for (int key = threadIdx.x; key < n; key += 256) {
+      const float w = wp[key];
+      float x = 0.f;
+      for (int h = 0; h < G; ++h) x = fmaf(weight_of(all_s[h * ws.ld + key], all_m[h], sc), all_r[h], x);
+      wp[key] = w + x;
     }
-    wp[key] = w + x;
   }
 }
 
@@ -895,6 +897,28 @@ __device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int rec
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// keys, values, positions and weights of `count` moves, by `threads` threads; no slot is both left and taken
+__device__ __forceinline__ void move_rows(const BoundedCache& c, int r, int kh, int row_pieces, const int2* moves, int count, int thread, int threads) {
+  const size_t rk = (size_t)r * c.Hkv + kh;
+  float* w = c.weight + rk * c.cap;
+  int32_t* q = c.pos + rk * c.cap;
+  for (int e = thread; e < count; e += threads) {
+    const int2 m = moves[e];
+    w[m.y] = w[m.x];
+    q[m.y] = q[m.x];
+  }
+  const int64_t total = (int64_t)count * row_pieces;
+  for (int64_t e = thread; e < total; e += threads) {
+    const int2 m = moves[e / row_pieces];
+    const int p = (int)(e % row_pieces);
+    const int64_t from = row_of_16(c, r, kh, m.x & ~15), to = row_of_16(c, r, kh, m.y & ~15);
+    if (from < 0 || to < 0) continue;
+    const int64_t a = (from + (m.x & 15)) * row_pieces + p, b = (to + (m.y & 15)) * row_pieces + p;
+    ((u32x4*)c.k)[b] = ((const u32x4*)c.k)[a];
+    ((u32x4*)c.v)[b] = ((const u32x4*)c.v)[a];
+  }
+}
+
 // exclusive sum of v over the workgroup's threads, the sum of all in total
 template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
@@ -908,15 +932,24 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
   return (u > 0 ? __builtin_amdgcn_readlane(w, u - 1) : 0) + incl - v;
 }
 
+// MOVE: the workgroup moves keys and values itself, from a list in LDS, and the row's last one sets its length (a ticket of the cache's, back at zero then; nothing
+// waits for it).  For caches that can hold few keys beyond the budget: a step's eviction is one launch.
+constexpr int MOVE_MOST = 64;
 // IN_LDS: the ranks stay on chip, slot i at i + i / 32 (a thread's slots lie side by side, threads' on different banks), otherwise they are made again from
 // weights and positions each time
-template <bool IN_LDS>
-__global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, EvictWs ws) {
+template <bool IN_LDS, bool MOVE>
+__global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, int row_pieces, EvictWs ws) {
   constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS, FEW = 4;
   const int r = blockIdx.y, kh = blockIdx.x, n = held_keys(c, r);
   const size_t rk = (size_t)r * c.Hkv + kh;
+  auto leave = [&]() {                                             // (MOVE; in front of it every wave has read the length, or has one that stays as it is)
+    if (threadIdx.x != 0 || atomicAdd(&c.tickets[r], 1) != c.Hkv - 1) return;
+    c.len[r] = min(n, budget);
+    __hip_atomic_store(&c.tickets[r], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
   if (n <= budget) {
-    if (threadIdx.x == 0) ws.counts[rk] = 0;
+    if (MOVE) leave();
+    else if (threadIdx.x == 0) ws.counts[rk] = 0;
     return;
   }
   float* wp = c.weight + rk * c.cap;
@@ -1022,7 +1055,8 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
     }
   }
   // in the order of slots, four a thread and turn: which stay, and the i-th hole in front of `budget` gets the i-th that stays behind it
-  int2* moves = ws.moves + rk * ws.most;
+  __shared__ int2 sh_moves[MOVE ? MOVE_MOST : 1];
+  int2* moves = MOVE ? sh_moves : ws.moves + rk * ws.most;
   int equal0 = 0, holes0 = 0, movers0 = 0;
   for (int base = 0; base < n; base += 4 * THREADS) {
     const int i0 = base + 4 * threadIdx.x;
@@ -1051,31 +1085,19 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
     }
     equal0 += all_equal; holes0 += all >> 16; movers0 += all & 0xffff;
   }
-  if (threadIdx.x == 0) ws.counts[rk] = movers0;
+  if constexpr (MOVE) {
+    __syncthreads();
+    move_rows(c, r, kh, row_pieces, sh_moves, movers0, threadIdx.x, THREADS);
+    leave();
+  } else {
+    if (threadIdx.x == 0) ws.counts[rk] = movers0;
+  }
 }
 
 __global__ __launch_bounds__(256) void evict_move_kernel(BoundedCache c, int budget, int row_pieces, EvictWs ws) {
   const int r = blockIdx.y / c.Hkv, kh = blockIdx.y % c.Hkv;
   if (blockIdx.x == 0 && kh == 0 && threadIdx.x == 0) c.len[r] = min(held_keys(c, r), budget);       // (nothing else of this launch reads it)
-  const int count = ws.counts[blockIdx.y];
-  const int64_t total = (int64_t)count * row_pieces;
-  const int2* moves = ws.moves + (size_t)blockIdx.y * ws.most;
-  float* w = c.weight + (size_t)blockIdx.y * c.cap;
-  int32_t* q = c.pos + (size_t)blockIdx.y * c.cap;
-  for (int e = blockIdx.x * 256 + threadIdx.x; e < count; e += gridDim.x * 256) {
-    const int2 m = moves[e];
-    w[m.y] = w[m.x];
-    q[m.y] = q[m.x];
-  }
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-    const int2 m = moves[e / row_pieces];
-    const int p = (int)(e % row_pieces);
-    const int64_t from = row_of_16(c, r, kh, m.x & ~15), to = row_of_16(c, r, kh, m.y & ~15);
-    if (from < 0 || to < 0) continue;
-    const int64_t a = (from + (m.x & 15)) * row_pieces + p, b = (to + (m.y & 15)) * row_pieces + p;
-    ((u32x4*)c.k)[b] = ((const u32x4*)c.k)[a];
-    ((u32x4*)c.v)[b] = ((const u32x4*)c.v)[a];
-  }
+  move_rows(c, r, kh, row_pieces, ws.moves + (size_t)blockIdx.y * ws.most, ws.counts[blockIdx.y], blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
@@ -1103,14 +1125,15 @@ int by_head(int D, F&& f) {                              // (mi_op_bounded_* hav
   return fail(MI_ERR_UNSUPPORTED, "bounded cache: head_dim");
 }
 
-// Slices of a row's keys; one: the kernel needs no joining launch, and its workgroups take all query heads of a KV head, 16 at a time.  That is for short caches: 321 keys of 8 KV
-// heads 8.7 us, in slices 10.8.  Otherwise four workgroups a CU, for long caches two: 32 rows of up to 2048 keys 44.0 us with four, 47.4 with two, 46.8 with eight; 4 of 32761 keys
-// 120, 117, 126.
+// 321 keys of 8 KV heads: 8.7 us alone, in slices 10.8
+bool attend_alone(const BoundedCache& c, int Hq) {
+  const int G = Hq / c.Hkv;
+  return c.cap <= 512 && c.cap * ((G + 15) / 16) <= 1024 && ((c.cap + 31) & ~31) * G <= ALONE_SCORES;
+}
+// Slices of a row's keys: four workgroups a CU, for long caches two: 32 rows of up to 2048 keys 44.0 us with four, 47.4 with two, 46.8 with eight; 4 of 32761 keys 120, 117, 126.
 int attend_splits(const BoundedCache& c, int Hq, int ncu) {
-  const int groups = (Hq / c.Hkv + 15) / 16, tiles = c.rows * c.Hkv * groups;
-  if (c.cap <= 512 && c.cap * groups <= 1024) return 1;
-  const int wgs = c.cap >= 16384 ? 2 : 4;
-  return std::max(groups > 1 ? 2 : 1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
+  const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16), wgs = c.cap >= 16384 ? 2 : 4;
+  return std::max(1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
 }
 // How a call is cut: units of nearly equal size, several times as many as the chip holds at once, so that its queues even them out.  First pass: 64 U queries by
 // `chunk` keys; second: 64 KS keys by `per` tiles of queries.
@@ -1140,6 +1163,7 @@ bool bounded_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 96 |
 bool bounded_group(int G) { return G >= 1 && G <= MAX_GROUP; }
 
 size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
+  if (attend_alone(c, Hq)) return 0;
   const size_t splits = attend_splits(c, Hq, ncu), ld = ((size_t)c.cap + 31) & ~(size_t)31;
   return up256((size_t)c.rows * Hq * ld * 4) + up256((size_t)c.rows * Hq * splits * 8) + up256((size_t)c.rows * Hq * splits * c.D * 4);
 }
@@ -1149,7 +1173,8 @@ size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   return one + std::max(p.splits > 1 ? one * p.splits : 0, p.slices > 1 ? (size_t)p.slices * c.rows * c.Hkv * ld * 4 : 0);
 }
 size_t bounded_evict_ws(const BoundedCache& c, int budget) {
-  return up256((size_t)c.rows * c.Hkv * 4) + up256((size_t)c.rows * c.Hkv * std::max(0, std::min(budget, c.cap - budget)) * 8);
+  const int most = std::min(budget, c.cap - budget);
+  return most <= MOVE_MOST ? 0 : up256((size_t)c.rows * c.Hkv * 4) + up256((size_t)c.rows * c.Hkv * most * 8);
 }
 
 int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStream_t st) {
@@ -1179,10 +1204,13 @@ int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* w
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
     return by_head(c.D, [&](auto e) {
-      const dim3 grid(splits, c.rows * c.Hkv, splits > 1 ? (G + 15) / 16 : 1);
-      hipLaunchKernelGGL((attend_kernel<T, decltype(e)::value>), grid, dim3(256), 0, st, c, a, w, splits);
-      if (splits > 1)
+      constexpr int E = decltype(e)::value;
+      if (attend_alone(c, a.Hq)) {
+        hipLaunchKernelGGL((attend_kernel<T, E, true>), dim3(1, c.rows * c.Hkv), dim3(256), 0, st, c, a, w, 1);
+      } else {
+        hipLaunchKernelGGL((attend_kernel<T, E, false>), dim3(splits, c.rows * c.Hkv, (G + 15) / 16), dim3(256), 0, st, c, a, w, splits);
         hipLaunchKernelGGL((attend_join_kernel<T>), dim3((c.cap + JOIN_KEYS - 1) / JOIN_KEYS, c.rows * c.Hkv), dim3(256), 0, st, c, a, w, splits);
+      }
       MI_HIP(hipGetLastError());
       return MI_OK;
     });
@@ -1217,14 +1245,17 @@ int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int 
   if (budget >= c.cap) return MI_OK;                     // no row can hold more
   const EvictWs w{(int32_t*)ws, (int2*)((char*)ws + up256((size_t)c.rows * c.Hkv * 4)), std::min(budget, c.cap - budget)};
   const dim3 grid(c.Hkv, c.rows);
-  const size_t lds = ((size_t)c.cap + c.cap / 32 + 1) * 4;
-  if (c.cap <= 12288)                               // ranks in LDS: 50 KiB
-    hipLaunchKernelGGL((evict_select_kernel<true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, w);
-  else
-    hipLaunchKernelGGL((evict_select_kernel<false>), grid, dim3(1024), 0, st, c, budget, keep_first, keep_last, w);
   const int pieces = c.D * (int)dtype_size(c.dtype) / 16;
-  const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(64, ((int64_t)w.most * pieces + 1023) / 1024));
-  hipLaunchKernelGGL(evict_move_kernel, dim3(groups, c.rows * c.Hkv), dim3(256), 0, st, c, budget, pieces, w);
+  const bool on_chip = c.cap <= 12288, move = w.most <= MOVE_MOST;         // ranks in LDS: 50 KiB
+  const size_t lds = on_chip ? ((size_t)c.cap + c.cap / 32 + 1) * 4 : 0;
+  if (on_chip && move) hipLaunchKernelGGL((evict_select_kernel<true, true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+  else if (on_chip) hipLaunchKernelGGL((evict_select_kernel<true, false>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+  else if (move) hipLaunchKernelGGL((evict_select_kernel<false, true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+  else hipLaunchKernelGGL((evict_select_kernel<false, false>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+  if (!move) {
+    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(64, ((int64_t)w.most * pieces + 1023) / 1024));
+    hipLaunchKernelGGL(evict_move_kernel, dim3(groups, c.rows * c.Hkv), dim3(256), 0, st, c, budget, pieces, w);
+  }
   MI_HIP(hipGetLastError());
   return MI_OK;
 }

@@ -467,6 +467,7 @@ struct BoundedCache {
   const int32_t* btab;
   int32_t* len; int32_t* next;             // [rows] slots filled, position of the next token
   int32_t* pos; float* weight;             // [rows][Hkv][cap]
+  int32_t* tickets;                        // [rows] zero between calls
 };
 struct BoundedTokens {
   const void* qkv; int64_t ld_row, ld_token;

@@ -50,9 +50,9 @@ int bounded_cache(const mi_op_bounded_cache* c, bool pointers, BoundedCache& o) 
     return fail(MI_ERR_INVALID, "mi_op_bounded: rows, KV heads (at most 65535 together) and slots");
   if (c->dtype != MI_F32 && c->dtype != MI_BF16 && c->dtype != MI_F16) return fail(MI_ERR_INVALID, "mi_op_bounded: dtype");
   if (!bounded_head_dim(c->D)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded: head sizes 16, 32, 64, 96, 128, 192 and 256");
-  o = BoundedCache{c->rows, c->Hkv, c->D, c->dtype, c->cap, c->n_blocks, c->bt_stride, c->bs_shift, c->k, c->v, c->btab, c->len, c->next, c->pos, c->weight};
+  o = BoundedCache{c->rows, c->Hkv, c->D, c->dtype, c->cap, c->n_blocks, c->bt_stride, c->bs_shift, c->k, c->v, c->btab, c->len, c->next, c->pos, c->weight, c->tickets};
   if (!pointers) return MI_OK;
-  if (!c->k || !c->v || !c->len || !c->next || !c->pos || !c->weight) return fail(MI_ERR_INVALID, "mi_op_bounded: null array");
+  if (!c->k || !c->v || !c->len || !c->next || !c->pos || !c->weight || !c->tickets) return fail(MI_ERR_INVALID, "mi_op_bounded: null array");
   if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded: keys and values are aligned to 16 bytes");
   if (c->btab && (c->bs_shift < 4 || c->bs_shift > 20 || c->n_blocks < 1 || c->bt_stride < 1 || (int64_t)c->bt_stride << c->bs_shift < c->cap))
     return fail(MI_ERR_INVALID, "mi_op_bounded: blocks of a power of two of tokens from 16 on, and a table that reaches to the last slot");

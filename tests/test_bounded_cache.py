@@ -17,7 +17,7 @@ P = (C.addressof(SOME) + 15) & ~15                       # (never read)
 
 def cache(**kw):
     c = L.OpBoundedCache()
-    for n, v in dict(dict(rows=2, Hkv=2, D=64, dtype=L.MI_BF16, cap=100, k=P, v=P, len=P, next=P, pos=P, weight=P), **kw).items():
+    for n, v in dict(dict(rows=2, Hkv=2, D=64, dtype=L.MI_BF16, cap=100, k=P, v=P, len=P, next=P, pos=P, weight=P, tickets=P), **kw).items():
         setattr(c, n, v)
     return C.byref(c)
 
@@ -40,7 +40,7 @@ PAGED = dict(btab=P, n_blocks=10, bt_stride=7, bs_shift=4)
 @pytest.mark.parametrize("change,code,text", [
     (dict(rows=0), -1, "rows"), (dict(rows=70000), -1, "rows"), (dict(rows=40000, Hkv=2), -1, "rows"), (dict(Hkv=0), -1, "rows"), (dict(cap=0), -1, "slots"),
     (dict(dtype=3), -1, "dtype"), (dict(D=80), -3, "head sizes"), (dict(D=512), -3, "head sizes"), (dict(k=None), -1, "null"), (dict(weight=None), -1, "null"),
-    (dict(len=None), -1, "null"), (dict(k=P + 2), -1, "aligned"), (dict(PAGED, bs_shift=3), -1, "blocks"), (dict(PAGED, n_blocks=0), -1, "blocks"),
+    (dict(len=None), -1, "null"), (dict(tickets=None), -1, "null"), (dict(k=P + 2), -1, "aligned"), (dict(PAGED, bs_shift=3), -1, "blocks"), (dict(PAGED, n_blocks=0), -1, "blocks"),
     (dict(PAGED, bt_stride=6), -1, "blocks"), (dict(PAGED, bs_shift=30), -1, "blocks")])
 def test_caches_that_every_call_refuses(change, code, text):
     lib, c = L.lib(), cache(**change)
@@ -73,9 +73,9 @@ def test_attend_weigh_and_evict_refuse():
 
 def test_sizes_of_workspaces_need_no_device():
     lib = L.lib()
-    assert lib.mi_op_bounded_attend_ws(cache(k=None), 4) > 2 * 4 * 100 * 4
+    assert lib.mi_op_bounded_attend_ws(cache(k=None, cap=1000), 4) > 2 * 4 * 1000 * 4 and lib.mi_op_bounded_attend_ws(cache(), 4) == 0
     assert lib.mi_op_bounded_weigh_ws(cache(), 50, 4, 0) >= 2 * 4 * 50 * 8
-    assert lib.mi_op_bounded_evict_ws(cache(), 30) >= 2 * 2 * 30 * 8
+    assert lib.mi_op_bounded_evict_ws(cache(cap=1000), 300) >= 2 * 2 * 300 * 8 and lib.mi_op_bounded_evict_ws(cache(), 90) == 0
     assert lib.mi_op_bounded_attend_ws(cache(D=80), 4) == 0 and lib.mi_op_bounded_attend_ws(cache(), 3) == 0
 
 

@@ -574,6 +574,18 @@ def test_two_streams_at_once():
         assert all(torch.equal(a, b) for a, b in zip(outs[i], want))
 
 
+def test_a_new_cache_on_another_stream():
+    """A cache made on one stream and evicted from at once on another, many heads racing for the row's ticket; the tickets are back at zero."""
+    s = Setup(75, 40, 16, 16, 90, [90 - r for r in range(40)], "float32")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for budget in (60, 59, 58, 30):
+            evict_once(s, budget, 4, 8)
+    torch.cuda.synchronize()
+    assert s.cache._tickets.tolist() == [0] * 40
+
+
 def test_the_same_call_twice_gives_the_same_bits():
     s = Setup(74, 3, 2, 128, 2000, [2000, 1500, 77], "bfloat16", True)
     a, b = copies(s), copies(s)
