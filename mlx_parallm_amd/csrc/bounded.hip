@@ -545,8 +545,10 @@ __device__ __forceinline__ WeighPlace weigh_place(const BoundedCache& c, int sli
 template <typename T>
 constexpr int weigh_queries() { return sizeof(T) == 4 ? 64 : 128; }
 
-template <typename T, int E>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_stats_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits, int chunk) {
+// ALONE: a workgroup holds all queries of a KV head (few of them, before few keys) and walks the keys twice, statistics first, then weights, summed over its columns: one launch, no
+// workspace.
+template <typename T, int E, bool ALONE>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 && !ALONE ? 3 : 2) void weigh_stats_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits, int chunk) {
   constexpr int D = 16 * E, ROWS = tile_rows<T, D>(), QUERIES = weigh_queries<T>(), U = QUERIES / 64;
   using St = Stage<T, D, ROWS>;
   const int G = a.Hq / c.Hkv;
@@ -559,6 +561,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
   __shared__ __align__(16) char tiles[2][ROWS * St::LD];
   __shared__ bool lost[2][ROWS / 16];
+  __shared__ float sums[ALONE ? 2 : 1][4][ROWS];
 
   Frag<T, D> q[U];
   int sees[U];                                           // keys that the column's query sees
@@ -618,81 +621,105 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
         if ((threadIdx.x + s * 256) % (16 * St::PER) == 0) lost[buf][St::row(s) / 16] = gone[s];
     }
   };
-  if (s0 < s1) {
-    look(s0);
-    fetch(s0);
-    look(s0 + ROWS);
-    put(0);
-  }
-  __syncthreads();
-  int cur = 0;
-  for (int base = s0; base < s1; base += ROWS, cur ^= 1) {
-    const bool more = base + ROWS < s1;
-    if (more) {
-      fetch(base + ROWS);
-      look(base + 2 * ROWS);
+  float inv[U];
+  auto walk = [&](auto second) {
+    if (s0 < s1) {
+      look(s0);
+      fetch(s0);
+      look(s0 + ROWS);
+      put(0);
     }
-    const char* tile = tiles[cur];
-    bool edge = base + ROWS > min(all, s1);
-    if (table != nullptr) {
+    __syncthreads();
+    int cur = 0;
+    for (int base = s0; base < s1; base += ROWS, cur ^= 1) {
+      const bool more = base + ROWS < s1;
+      if (more) {
+        fetch(base + ROWS);
+        look(base + 2 * ROWS);
+      }
+      const char* tile = tiles[cur];
+      bool edge = base + ROWS > min(all, s1);
+      if (table != nullptr) {
 #pragma unroll
-      for (int t = 0; t < ROWS / 16; ++t) edge = edge || lost[cur][t];
-    }
-    // 32 keys at a time; their products run while the exponentials of the 32 in front of them do
-    auto keys = [&](auto masked) {
-      f32x4 sv[2][2][U];
-      auto products = [&](int t0, f32x4 (&o)[2][U]) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          Frag<T, D> k;
-          k.load((const T*)(tile + ((t0 + t) * 16 + ln) * St::LD), qd);
-#pragma unroll
-          for (int u = 0; u < U; ++u) o[t][u] = dot16(k, q[u]);
-        }
-      };
-      products(0, sv[0]);
-#pragma unroll
-      for (int t0 = 0; t0 < ROWS / 16; t0 += 2) {
-        if (t0 + 2 < ROWS / 16) products(t0 + 2, sv[(t0 / 2 + 1) & 1]);
-        f32x4 (&s)[2][U] = sv[(t0 / 2) & 1];
-        if constexpr (decltype(masked)::value) {
+        for (int t = 0; t < ROWS / 16; ++t) edge = edge || lost[cur][t];
+      }
+      // 32 keys at a time; their products run while the exponentials of the 32 in front of them do
+      auto keys = [&](auto masked) {
+        f32x4 sv[2][2][U];
+        auto products = [&](int t0, f32x4 (&o)[2][U]) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            const int key = base + (t0 + t) * 16 + 4 * qd;
-            const bool there = table == nullptr || !lost[cur][t0 + t];
+            Frag<T, D> k;
+            k.load((const T*)(tile + ((t0 + t) * 16 + ln) * St::LD), qd);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int left = there ? min(sees[u], s1) - key : 0;
+            for (int u = 0; u < U; ++u) o[t][u] = dot16(k, q[u]);
+          }
+        };
+        products(0, sv[0]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (i >= left) s[t][u][i] = -INFINITY;
+        for (int t0 = 0; t0 < ROWS / 16; t0 += 2) {
+          if (t0 + 2 < ROWS / 16) products(t0 + 2, sv[(t0 / 2 + 1) & 1]);
+          f32x4 (&s)[2][U] = sv[(t0 / 2) & 1];
+          if constexpr (decltype(masked)::value) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int key = base + (t0 + t) * 16 + 4 * qd;
+              const bool there = table == nullptr || !lost[cur][t0 + t];
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                const int left = there ? min(sees[u], s1) - key : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (i >= left) s[t][u][i] = -INFINITY;
+              }
             }
           }
-        }
+          if constexpr (decltype(second)::value) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float top = s[0][u][0];
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+              for (int i = 0; i < 4; ++i) {
+                float x = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i]);
-          top = fmaxf(m[u], top);
-          float x = l[u] * weight_of(m[u], top, sc), y = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x += weight_of(s[0][u][i], top, sc);
-            y += weight_of(s[1][u][i], top, sc);
+                for (int u = 0; u < U; ++u) x = fmaf(weight_of(s[t][u][i], m[u], sc), inv[u], x);
+                x = row16_sum(x);
+                if (ln == 0) sums[cur][wave][(t0 + t) * 16 + 4 * qd + i] = x;
+              }
+            continue;
           }
-          m[u] = top; l[u] = x + y;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float top = s[0][u][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][u][i]);
+            top = fmaxf(m[u], top);
+            float x = l[u] * weight_of(m[u], top, sc), y = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x += weight_of(s[0][u][i], top, sc);
+              y += weight_of(s[1][u][i], top, sc);
+            }
+            m[u] = top; l[u] = x + y;
+          }
+          if constexpr (sizeof(T) == 2 && !decltype(masked)::value) interleave<2 * U * Frag<T, D>::N, 3, 1>();
         }
-        if constexpr (sizeof(T) == 2 && !decltype(masked)::value) interleave<2 * U * Frag<T, D>::N, 3, 1>();
+      };
+      if (edge) keys(std::true_type{});
+      else keys(std::false_type{});
+      const bool there = (int)threadIdx.x < ROWS && base + (int)threadIdx.x < s1 && (table == nullptr || !lost[cur][threadIdx.x / 16]);
+      if (more) put(cur ^ 1);
+      __syncthreads();
+      if constexpr (decltype(second)::value) {
+        if (there) {
+          float* wp = c.weight + ((size_t)r * c.Hkv + kh) * c.cap + base + threadIdx.x;
+          *wp += (sums[cur][0][threadIdx.x] + sums[cur][1][threadIdx.x]) + (sums[cur][2][threadIdx.x] + sums[cur][3][threadIdx.x]);
+        }
       }
-    };
-    if (edge) keys(std::true_type{});
-    else keys(std::false_type{});
-    if (more) put(cur ^ 1);
-    __syncthreads();
-  }
+    }
+  };
+  walk(std::false_type{});
 #pragma unroll
   for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -700,6 +727,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
       const float mo = __shfl_xor(m[u], off, 64), lo = __shfl_xor(l[u], off, 64), M = fmaxf(m[u], mo);
       l[u] = l[u] * weight_of(m[u], M, sc) + lo * weight_of(mo, M, sc);
       m[u] = M;
+    }
+    if constexpr (ALONE) {
+      inv[u] = l[u] != 0.f ? 1.f / l[u] : 0.f;
+      continue;
     }
     const int rho = rho0 + (wave * U + u) * 16 + ln;
     if (qd == 0 && rho < rhos) {
@@ -713,6 +744,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_s
       }
     }
   }
+  if constexpr (ALONE) walk(std::true_type{});
 }
 
 __global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, BoundedWeigh a, WeighWs ws, int splits, int chunk, int queries) {
@@ -1135,6 +1167,16 @@ int attend_splits(const BoundedCache& c, int Hq, int ncu) {
   const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16), wgs = c.cap >= 16384 ? 2 : 4;
   return std::max(1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
 }
+// All queries of a KV head in one workgroup: where there are few of them, before few keys or in rows and heads enough to fill the chip.  us, alone / in units: 30 queries of 30 keys 7.3 /
+// 12.3, 32 of 256 15.2 / 17.6, 32 of 400 23.3 / 17.3; float32 16 of 100 16.8 / 17.8, of 200 26.1 / 21.8; 64 rows of 8 heads, 32 queries, 400 keys 36 / 61, 4000 keys 294 / 407, float32 16 of 400 84 / 153;
+// 256 rows and heads of 1000 keys 53 / 58; 200 of 300 keys, 3 queries, 18 / 52.
+bool weigh_alone(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  const bool f32 = c.dtype == MI_F32;
+  const int64_t L = a.last > 0 ? std::min(a.last, a.L) : a.L;
+  if (L * (a.Hq / c.Hkv) > (f32 ? weigh_queries<float>() : weigh_queries<bf16>())) return false;
+  return c.cap <= (f32 ? 128 : 288) || 4 * c.rows * c.Hkv >= 3 * ncu;
+}
+
 // How a call is cut: units of nearly equal size, several times as many as the chip holds at once, so that its queues even them out.  First pass: 64 U queries by
 // `chunk` keys; second: 64 KS keys by `per` tiles of queries.
 struct WeighPlan { int splits, chunk, ks, per, slices; };
@@ -1168,6 +1210,7 @@ size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
   return up256((size_t)c.rows * Hq * ld * 4) + up256((size_t)c.rows * Hq * splits * 8) + up256((size_t)c.rows * Hq * splits * c.D * 4);
 }
 size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  if (weigh_alone(c, a, ncu)) return 0;
   const WeighPlan p = weigh_plan(c, a, ncu);
   const size_t one = up256((size_t)c.rows * a.Hq * a.L * 8), ld = ((size_t)c.cap + 3) & ~(size_t)3;
   return one + std::max(p.splits > 1 ? one * p.splits : 0, p.slices > 1 ? (size_t)p.slices * c.rows * c.Hkv * ld * 4 : 0);
@@ -1229,7 +1272,12 @@ int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws,
       constexpr int E = decltype(e)::value;
       constexpr int Q = weigh_queries<T>(), KS = sizeof(T) == 4 ? 1 : 2;
       const dim3 queries((rhos + Q - 1) / Q * p.splits * pairs), keys((c.cap + 64 * p.ks - 1) / (64 * p.ks) * p.slices * pairs);
-      hipLaunchKernelGGL((weigh_stats_kernel<T, E>), queries, dim3(256), 0, st, c, a, w, p.splits, p.chunk);
+      if (weigh_alone(c, a, ncu)) {
+        hipLaunchKernelGGL((weigh_stats_kernel<T, E, true>), dim3(pairs), dim3(256), 0, st, c, a, w, 1, c.cap);
+        MI_HIP(hipGetLastError());
+        return MI_OK;
+      }
+      hipLaunchKernelGGL((weigh_stats_kernel<T, E, false>), queries, dim3(256), 0, st, c, a, w, p.splits, p.chunk);
       if (p.splits > 1) hipLaunchKernelGGL(weigh_merge_kernel, dim3((rhos + 255) / 256, pairs), dim3(256), 0, st, c, a, w, p.splits, p.chunk, Q);
       if (p.ks == KS) hipLaunchKernelGGL((weigh_add_kernel<T, E, KS>), keys, dim3(256), 0, st, c, a, w, p.per, p.slices);
       else hipLaunchKernelGGL((weigh_add_kernel<T, E, 1>), keys, dim3(256), 0, st, c, a, w, p.per, p.slices);

@@ -74,7 +74,7 @@ def test_attend_weigh_and_evict_refuse():
 def test_sizes_of_workspaces_need_no_device():
     lib = L.lib()
     assert lib.mi_op_bounded_attend_ws(cache(k=None, cap=1000), 4) > 2 * 4 * 1000 * 4 and lib.mi_op_bounded_attend_ws(cache(), 4) == 0
-    assert lib.mi_op_bounded_weigh_ws(cache(), 50, 4, 0) >= 2 * 4 * 50 * 8
+    assert lib.mi_op_bounded_weigh_ws(cache(), 150, 4, 0) >= 2 * 4 * 150 * 8 and lib.mi_op_bounded_weigh_ws(cache(), 50, 4, 0) == 0
     assert lib.mi_op_bounded_evict_ws(cache(cap=1000), 300) >= 2 * 2 * 300 * 8 and lib.mi_op_bounded_evict_ws(cache(), 90) == 0
     assert lib.mi_op_bounded_attend_ws(cache(D=80), 4) == 0 and lib.mi_op_bounded_attend_ws(cache(), 3) == 0
 

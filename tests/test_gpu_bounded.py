@@ -340,6 +340,20 @@ def test_weigh_more_queries_than_slots():
     weigh_once(Setup(41, 3, 1, 64, 64, [64, 20, 0], "bfloat16", True, bad=3), 50, 4)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D", [16, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("L,G", [(1, 1), (7, 3), (16, 4), (3, 16)])
+def test_weigh_few_queries(L, G, D, dtype):
+    """One workgroup a row and head: few keys; pages that are none; rows with fewer keys than queries."""
+    weigh_once(Setup(L + D, 3, 2, D, 120, [120, 65, 2], dtype, True, bad=4), L, 2 * G)
+    weigh_once(Setup(L + D + 1, 2, 1, D, 128, [128, 0], dtype), L, G, counts=[L, max(0, L - 1)], last=2)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_weigh_few_queries_of_many_rows(dtype):
+    weigh_once(Setup(43, 100, 2, 32, 400, [400 - 3 * r for r in range(100)], dtype, True), 5, 4, counts=[r % 6 for r in range(100)])
+
+
 def test_weigh_many_rows():
     weigh_once(Setup(42, 40, 2, 16, 70, [70 - r for r in range(40)], "float32"), 9, 4)
 
