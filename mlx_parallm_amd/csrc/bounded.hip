@@ -476,7 +476,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 // other way round.
 // Bound by the matrix cores and the exponentials beside them, which hardly overlap: a block of 64 scores costs 16 cycles of the one and 15 to 20 of the other at D = 128.  4 prompts of 819 to 2048 bf16
 // tokens, 32 / 8 heads: 64 + 71 + 5 us, 2 x 37 GFLOP, 560 TFLOP/s over both passes (a product of 8192 x 8192 x 8192: 1135; the clock under this load is 1.95 GHz).  2 prompts of 700 float32 tokens 58 + 5
-// + 56 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
+// + 57 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
 // Workspace: [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
 // queries, [slice][row][KV head][ld] sums.
 struct WeighWs { float* stats; float* parts; float* sums; int ld; };
@@ -917,7 +917,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 // above all): a histogram over the range that is left, 2048 bins, until a bin stays whole -- at most three, one or two where the weights differ.  A
 // second launch moves keys and values: with the moves known it spreads over the chip.
 // 64 rows and heads of 8192 keys down to 1024: 12.8 us (a chain of barriers on 64 CUs; the first histogram's range is wasted on the gap between zero and the least weight) + 15 us to move 59 MB (3.9 TB/s in rows of
-// 256 bytes); 256 of 1025 down to 1024: 6.5 + 3.
+// 256 bytes); 256 of 1025 down to 1024, in one launch: 8.5.
 struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
 
 // Where more keys are protected than the budget holds, they alone are ranked (`crowded`).
@@ -965,13 +965,13 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
 }
 
 // MOVE: the workgroup moves keys and values itself, from a list in LDS, and the row's last one sets its length (a ticket of the cache's, back at zero then; nothing
-// waits for it).  For caches that can hold few keys beyond the budget: a step's eviction is one launch.
+// waits for it).  For caches that can hold few keys beyond the budget: a step's eviction is one launch (32 rows of 8 heads, 1025 keys to 1024: 8.5 us, in two 6.5 + 3 and 3 us more of host time).
 constexpr int MOVE_MOST = 64;
 // IN_LDS: the ranks stay on chip, slot i at i + i / 32 (a thread's slots lie side by side, threads' on different banks), otherwise they are made again from
 // weights and positions each time
 template <bool IN_LDS, bool MOVE>
 __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, int row_pieces, EvictWs ws) {
-  constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS, FEW = 4;
+  constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS, FEW = 4;       // (256 threads: 12.4 us for 8.8)
   const int r = blockIdx.y, kh = blockIdx.x, n = held_keys(c, r);
   const size_t rk = (size_t)r * c.Hkv + kh;
   auto leave = [&]() {                                             // (MOVE; in front of it every wave has read the length, or has one that stays as it is)
@@ -1033,7 +1033,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   uint32_t cut = RANK_STAYS - 1;
   int need = 0;
   bool found = false;
-  if (n - budget <= FEW && !crowded) {                             // few leave: the least weighted alone (always, where it is one key a step)
+  if (n - budget <= FEW && !crowded) {                             // few leave: the least weighted alone (always, where it is one key a step; 9.8 -> 6.5 us of selection)
     int equal = 0, all;
     for (int i = threadIdx.x; i < n; i += THREADS) equal += rank(i) == lo;
     block_scan<THREADS>(equal, all, scan);
@@ -1190,7 +1190,7 @@ WeighPlan weigh_plan(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   auto key_tiles = [&](int ks) { return pairs * ((c.cap + 64 * ks - 1) / (64 * ks)); };
   p.ks = !f32 && key_tiles(2) >= ncu ? 2 : 1;
   const int rows = c.D * (int)dtype_size(c.dtype) <= 256 ? 64 : 32;
-  const int64_t tiles = (int64_t)G * ((L + rows - 1) / rows), least = f32 ? 2 : 8;
+  const int64_t tiles = (int64_t)G * ((L + rows - 1) / rows), least = f32 ? 4 : 8;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({MAX_SPLITS, 24 * ncu / key_tiles(p.ks), (tiles + least - 1) / least}));
   p.per = (int)((tiles + want - 1) / want);
   p.slices = (int)((tiles + p.per - 1) / p.per);
