@@ -1,4 +1,4 @@
-"""A cache of fixed size in 64-bit NumPy, slot by slot (the checker of mlx_parallm_amd.bounded_cache)."""
+"""A cache of fixed size in 64-bit NumPy, slot by slot (what mlx_parallm_amd.bounded_cache is tested against)."""
 from __future__ import annotations
 
 import numpy as np
