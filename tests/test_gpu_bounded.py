@@ -147,6 +147,38 @@ def test_append_takes_what_fits(L):
         assert np.array_equal(f64(x)[~belongs], f64(y)[~belongs], equal_nan=True)
 
 
+def test_counts_beyond_the_tokens_and_below_none():
+    s = Setup(4, 3, 2, 32, 90, [10, 20, 30], "float32")
+    cos, sin = angles(200, 32)
+    counts = torch.tensor([7, -3, 2 ** 31 - 1], dtype=torch.int32)
+    qkv = s.randn(3, 5, 8 * 32)
+    q = s.cache.append(qkv.cuda(), 4, cos.cuda(), sin.cuda(), counts=counts.cuda())
+    want, dq, _ = s.model.append(f64(qkv), 4, cos.numpy(), sin.numpy(), counts.numpy())
+    within(f64(q), want, dq + (np.abs(want) + dq) * HALF["float32"])
+    s.check_meta()
+    s.model.k, s.model.v = s.caches()
+    weigh_once(s, 5, 4, counts=counts.tolist())
+    attend_once(s, 4, counts=counts.tolist())
+
+
+def test_queries_in_other_strides_and_places():
+    s = Setup(6, 2, 2, 64, 100, [100, 60], "bfloat16")
+    a, b = copies(s), copies(s)
+    wide = s.randn(2, 8, 3, 64).cuda()
+    q = wide[:, :, 1]
+    assert torch.equal(a.attend(q), b.attend(q.contiguous())) and torch.equal(a.weights, b.weights)
+    p = s.randn(4, 2, 30, 64).cuda().permute(1, 2, 0, 3)                # [rows][tokens][heads][D]
+    a.weigh(p)
+    b.weigh(p.contiguous())
+    assert torch.equal(a.weights, b.weights)
+    odd = torch.zeros(2 * 8 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, 8, 64)
+    with pytest.raises(ValueError, match="16 bytes"):
+        a.attend(odd)
+    with pytest.raises(ValueError, match="16 bytes"):
+        a.append(torch.zeros((2, 1, 8 * 64 + 4), dtype=torch.bfloat16, device="cuda")[:, :, 4:], 4, *(t.cuda() for t in angles(10, 64)))
+    assert torch.equal(a.weights, b.weights)
+
+
 def test_append_strides():
     s = Setup(5, 2, 2, 32, 64, [3, 9], "float16")
     cos, sin = angles(64, 32)
@@ -297,6 +329,17 @@ def test_attend_beyond_32_bits():
     assert c.lengths.tolist() == [0, 100]
     assert torch.equal(torch.sort(c.positions[1, :, :100], 1).values, kept.int())
     assert torch.equal(c.keys[1, :, :100], torch.gather(k, 1, c.positions[1, :, :100, None].long().expand(-1, -1, 128)))
+    cos, sin = (t.cuda() for t in angles(400, 128))
+    for L in (1, 20):                                     # both forms of the append, then a prompt's weights
+        at = c.lengths[1].item()
+        qkv = torch.randn((2, L, 32 * 128), generator=g, device="cuda").bfloat16()
+        q = c.append(qkv, 16, cos, sin, counts=torch.tensor([0, L], dtype=torch.int32, device="cuda"))
+        assert torch.equal(c.values[1, :, at:at + L], qkv[1, :, 24 * 128:].view(L, 8, 128).transpose(0, 1))
+        want = c.weights[1, :, :at + L].double()
+        x = q[1].view(L, 8, 2, 128).permute(1, 2, 0, 3).double() @ c.keys[1, :, None, :at + L].double().transpose(-1, -2) / 128 ** 0.5
+        x.masked_fill_(torch.ones((L, at + L), dtype=torch.bool, device="cuda").triu(at + 1), -torch.inf)
+        c.weigh(q, counts=torch.tensor([0, L], dtype=torch.int32, device="cuda"))
+        torch.testing.assert_close(c.weights[1, :, :at + L].double(), want + torch.softmax(x, -1).sum((1, 2)), rtol=1e-4, atol=1e-6)
 
 
 # ---- weigh
