@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 // second launch moves keys and values: with the moves known it spreads over the chip.
 // 64 rows and heads of 8192 keys down to 1024: 12.8 us (a chain of barriers on 64 CUs; the first histogram's range is wasted on the gap between zero and the least weight) + 15 us to move 59 MB (3.9 TB/s in rows of
 // 256 bytes); 256 of 1025 down to 1024, in one launch: 8.5.
-struct EvictWs { int32_t* counts; int2* moves; int most; };       // [row][KV head]; [row][KV head][most] (from, to)
+struct EvictWs { int32_t* counts; int2* moves; uint32_t* ranks; int most; };      // [row][KV head]; [row][KV head][most] (from, to); [row][KV head][cap]
 
 // Where more keys are protected than the budget holds, they alone are ranked (`crowded`).
 constexpr uint32_t RANK_STAYS = 0xffffffffu, RANK_LEAVES = 0;
@@ -967,8 +967,9 @@ __device__ __forceinline__ int block_scan(int v, int& total, int* sh) {
 // MOVE: the workgroup moves keys and values itself, from a list in LDS, and the row's last one sets its length (a ticket of the cache's, back at zero then; nothing
 // waits for it).  For caches that can hold few keys beyond the budget: a step's eviction is one launch (32 rows of 8 heads, 1025 keys to 1024: 8.5 us, in two 6.5 + 3 and 3 us more of host time).
 constexpr int MOVE_MOST = 64;
-// IN_LDS: the ranks stay on chip, slot i at i + i / 32 (a thread's slots lie side by side, threads' on different banks), otherwise they are made again from
-// weights and positions each time
+// slots whose ranks fit the LDS of a CU: 149 KiB
+constexpr int ON_CHIP = 36864;      // (8 heads of 32768 keys down to 4096: 45 us; weights and positions read again at every sweep 70)
+// IN_LDS: the ranks stay on chip, slot i at i + i / 32 (a thread's slots lie side by side, threads' on different banks); otherwise they lie in the workspace
 template <bool IN_LDS, bool MOVE>
 __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int budget, int keep_first, int keep_last, int row_pieces, EvictWs ws) {
   constexpr int THREADS = 1024, BINS = 2048, PER = BINS / THREADS, FEW = 4;       // (256 threads: 12.4 us for 8.8)
@@ -987,13 +988,14 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   float* wp = c.weight + rk * c.cap;
   int32_t* pp = c.pos + rk * c.cap;
   const int recent_from = (int)max((int64_t)c.next[r] - keep_last, (int64_t)INT32_MIN);
-  extern __shared__ uint32_t ranks[];
+  extern __shared__ uint32_t lds_ranks[];
+  uint32_t* ranks = IN_LDS ? lds_ranks : ws.ranks + rk * c.cap;
   __shared__ uint32_t hist[BINS];
   __shared__ int scan[16];
   __shared__ uint32_t sh_lo[16], sh_hi[16];
   __shared__ int sh_prot[16], sh_bin, sh_above, sh_in;
   bool crowded = false;
-  auto rank = [&](int i) { return IN_LDS ? ranks[i + (i >> 5)] : rank_of(wp[i], pp[i], keep_first, recent_from, crowded); };
+  auto rank = [&](int i) -> uint32_t& { return IN_LDS ? lds_ranks[i + (i >> 5)] : ranks[i]; };
 
   // ranks, their range, and how many keys stay whatever their weight
   uint32_t lo, hi;
@@ -1010,7 +1012,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
         const int i = i0 + j * THREADS;
         if (i >= n) continue;
         const uint32_t k = rank_of(w[j], p[j], keep_first, recent_from, crowded);
-        if (IN_LDS) ranks[i + (i >> 5)] = k;
+        rank(i) = k;
         if (k == RANK_STAYS) ++prot;
         else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
       }
@@ -1047,12 +1049,13 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
     need = budget - prot;
     for (;;) {                                                     // the range [lo, hi] holds the rank; it shrinks by a factor of 1024 at least
       const int shift = max(0, 21 - __clz(hi - lo | 1u));
-      for (int i0 = threadIdx.x; i0 < n; i0 += 4 * THREADS) {
-        uint32_t k[4];
+      constexpr int BATCH = IN_LDS ? 4 : 16;
+      for (int i0 = threadIdx.x; i0 < n; i0 += BATCH * THREADS) {
+        uint32_t k[BATCH];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = rank(min(i0 + j * THREADS, n - 1));
+        for (int j = 0; j < BATCH; ++j) k[j] = rank(min(i0 + j * THREADS, n - 1));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < BATCH; ++j)
           if (i0 + j * THREADS < n && k[j] >= lo && k[j] <= hi) atomicAdd(&hist[(k[j] - lo) >> shift], 1u);
       }
       __syncthreads();
@@ -1090,14 +1093,21 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   __shared__ int2 sh_moves[MOVE ? MOVE_MOST : 1];
   int2* moves = MOVE ? sh_moves : ws.moves + rk * ws.most;
   int equal0 = 0, holes0 = 0, movers0 = 0;
+  uint32_t ahead[4];                                               // the next turn's
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ahead[j] = rank(min(4 * (int)threadIdx.x + j, n - 1));
   for (int base = 0; base < n; base += 4 * THREADS) {
     const int i0 = base + 4 * threadIdx.x;
     uint32_t k[4];
     int equal = 0, all_equal = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      k[j] = i0 + j < n ? rank(i0 + j) : 0;
+      k[j] = i0 + j < n ? ahead[j] : 0;
       if (i0 + j < n && k[j] == cut) ++equal;
+    }
+    if (base + 4 * THREADS < n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ahead[j] = rank(min(i0 + 4 * THREADS + j, n - 1));
     }
     int at = equal0 + (need > 0 ? block_scan<THREADS>(equal, all_equal, scan) : 0), both = 0, all;
     bool stays[4];
@@ -1217,7 +1227,9 @@ size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
 }
 size_t bounded_evict_ws(const BoundedCache& c, int budget) {
   const int most = std::min(budget, c.cap - budget);
-  return most <= MOVE_MOST ? 0 : up256((size_t)c.rows * c.Hkv * 4) + up256((size_t)c.rows * c.Hkv * most * 8);
+  if (most <= 0) return 0;                               // (no row can hold more)
+  const size_t pairs = (size_t)c.rows * c.Hkv;
+  return (most > MOVE_MOST ? up256(pairs * 4) + up256(pairs * most * 8) : 0) + (c.cap > ON_CHIP ? pairs * c.cap * 4 : 0);
 }
 
 int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStream_t st) {
@@ -1291,17 +1303,22 @@ int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws,
 
 int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int keep_last, void* ws, hipStream_t st) {
   if (budget >= c.cap) return MI_OK;                     // no row can hold more
-  const EvictWs w{(int32_t*)ws, (int2*)((char*)ws + up256((size_t)c.rows * c.Hkv * 4)), std::min(budget, c.cap - budget)};
+  const int most = std::min(budget, c.cap - budget);
+  const bool on_chip = c.cap <= ON_CHIP, move = most <= MOVE_MOST;
+  const size_t pairs = (size_t)c.rows * c.Hkv, counts = move ? 0 : up256(pairs * 4), moves = move ? 0 : up256(pairs * most * 8);
+  const EvictWs w{(int32_t*)ws, (int2*)((char*)ws + counts), (uint32_t*)((char*)ws + counts + moves), most};
   const dim3 grid(c.Hkv, c.rows);
   const int pieces = c.D * (int)dtype_size(c.dtype) / 16;
-  const bool on_chip = c.cap <= 12288, move = w.most <= MOVE_MOST;         // ranks in LDS: 50 KiB
   const size_t lds = on_chip ? ((size_t)c.cap + c.cap / 32 + 1) * 4 : 0;
-  if (on_chip && move) hipLaunchKernelGGL((evict_select_kernel<true, true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
-  else if (on_chip) hipLaunchKernelGGL((evict_select_kernel<true, false>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
-  else if (move) hipLaunchKernelGGL((evict_select_kernel<false, true>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
-  else hipLaunchKernelGGL((evict_select_kernel<false, false>), grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+  auto select = [&](auto kern) {
+    if (lds > 48 * 1024) MI_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kern, grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
+    return (int)MI_OK;
+  };
+  MI_TRY(on_chip ? (move ? select(evict_select_kernel<true, true>) : select(evict_select_kernel<true, false>))
+                 : (move ? select(evict_select_kernel<false, true>) : select(evict_select_kernel<false, false>)));
   if (!move) {
-    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(64, ((int64_t)w.most * pieces + 1023) / 1024));
+    const int groups = (int)std::max<int64_t>(1, std::min<int64_t>(64, ((int64_t)most * pieces + 1023) / 1024));
     hipLaunchKernelGGL(evict_move_kernel, dim3(groups, c.rows * c.Hkv), dim3(256), 0, st, c, budget, pieces, w);
   }
   MI_HIP(hipGetLastError());

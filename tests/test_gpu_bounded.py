@@ -423,7 +423,7 @@ def test_evict_types(dtype, D):
     evict_once(Setup(D, 2, 3, D, 130, [130, 100], dtype, True), 60, 2, 5)
 
 
-@pytest.mark.parametrize("n", [300, 5000, 13000])
+@pytest.mark.parametrize("n", [300, 5000, 13000, 37000])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "ties", "special", "negative", "near"])
 def test_evict_weights(kind, n):
     """All equal, mostly zero, many equal, NaN and infinities and both zeros, below zero, neighbouring numbers."""
@@ -440,10 +440,11 @@ def test_evict_weights(kind, n):
     evict_once(s, n // 3, 2, 9)
 
 
-def test_evict_large_caches():
-    """More slots than the selection holds on chip."""
-    s = Setup(77, 1, 2, 16, 40000, [39990], "bfloat16")
-    evict_once(s, 1000, 4, 64)
+@pytest.mark.parametrize("cap,n,budget", [(36864, 36860, 1000), (36865, 36865, 36800), (40000, 39990, 1000), (70000, 70000, 69999), (33000, 200, 100)])
+def test_evict_large_caches(cap, n, budget):
+    """On both sides of what the selection holds on chip, with much and little that moves."""
+    s = Setup(77, 1, 2, 16, cap, [n], "bfloat16")
+    evict_once(s, budget, 4, 64)
 
 
 def test_evict_all_protected_and_odd_positions():
@@ -454,6 +455,7 @@ def test_evict_all_protected_and_odd_positions():
     evict_once(s, 20, 4, 3)
     evict_once(Setup(55, 2, 1, 16, 90, [90, 60], "float32", skip=0), 20, 7, 2 ** 31 - 1)
     evict_once(Setup(56, 2, 2, 16, 15000, [15000, 14000], "float32", skip=0), 20, 30, 7)
+    evict_once(Setup(58, 2, 1, 16, 38000, [38000, 14000], "float32", skip=0), 20, 30, 7)
     s = Setup(57, 2, 1, 16, 90, [90, 60], "float32")
     s.cache.next_positions.fill_(-2 ** 31)
     s.model.next[:] = -2 ** 31
@@ -572,9 +574,10 @@ def same(a, b):
         assert torch.equal(getattr(a, x).nan_to_num(), getattr(b, x).nan_to_num()), x
 
 
-def test_captured_steps_are_the_eager_ones():
+@pytest.mark.parametrize("cap", [40, 1000, 20000])
+def test_captured_steps_are_the_eager_ones(cap):
     """A captured step, replayed with eager work of another cache in between."""
-    s = Setup(71, 4, 2, 64, 1000, [20, 3, 900, 0], "bfloat16")
+    s = Setup(71, 4, 2, 64, cap, [20, 3, cap - 10, 0], "bfloat16")
     cos, sin = (t.cuda() for t in angles(2000, 64))
     eager, other = copies(s), copies(s)
     x = torch.empty((4, 1, 12 * 64), dtype=torch.bfloat16, device="cuda")
