@@ -1311,7 +1311,8 @@ int launch_bounded_evict(const BoundedCache& c, int budget, int keep_first, int 
   const int pieces = c.D * (int)dtype_size(c.dtype) / 16;
   const size_t lds = on_chip ? ((size_t)c.cap + c.cap / 32 + 1) * 4 : 0;
   auto select = [&](auto kern) {
-    if (lds > 48 * 1024) MI_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    // (always the same limit: calls on other caches may set it in between)
+    if (lds > 48 * 1024) MI_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (ON_CHIP + ON_CHIP / 32 + 1) * 4));
     hipLaunchKernelGGL(kern, grid, dim3(1024), lds, st, c, budget, keep_first, keep_last, pieces, w);
     return (int)MI_OK;
   };
