@@ -178,7 +178,7 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // What a key weighs needs the final maximum and sum of every head, so the products are kept (4 bytes a head and key, 3 % of 16-bit keys and values at 4 heads) and read by whoever has
 // them: the workgroup itself where it is alone (`ALONE`), else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
 // Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
-// launches' heads; 8 rows of 1025 float32 keys, 68 MB, 20.7 + 4.8: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
+// launches' heads; 8 rows of 1025 float32 keys, 68 MB, 19.4 + 4.2: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
 
 // A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
 template <typename T, int D>
@@ -247,8 +247,15 @@ __device__ __forceinline__ void add_values(const Raw<E * 4> (&v)[4 * SUB], const
       for (int j = 0; j < E; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[4 * t + i].w[j]), p[t][i], o[j], 0, 0, 0);
 }
 
-// the slice of a row's keys that each of `splits` workgroups takes: a multiple of 128 (one tile of 32 for each of four waves)
-__device__ __forceinline__ int slice_keys(int n, int splits) { return ((n + splits - 1) / splits + 127) & ~127; }
+// Slices of a row's keys: at most `splits`, of a multiple of 128 keys each (one tile of 32 for each of four waves); up to 32 keys more are the last one's, not a slice of
+// their own.
+struct Slices { int keys, count; };
+__device__ __forceinline__ Slices slices_of(int n, int splits) {
+  Slices s;
+  s.keys = ((max(n - 32, 1) + splits - 1) / splits + 127) & ~127;
+  s.count = min(splits, (n + s.keys - 1) / s.keys);
+  return s;
+}
 
 // Short caches: one workgroup takes all keys and query heads of a KV head (16 at a time) and keeps the scores in LDS.  Otherwise slices and a joining launch.
 constexpr int ALONE_SCORES = 7168;                     // keys (in 32s) times heads: 28 KiB
@@ -267,8 +274,9 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ln = lane & 15, qd = lane >> 4;
   const bool idle = a.counts != nullptr && a.counts[r] <= 0;
   const int n = idle ? 0 : held_keys(c, r);
-  const int chunk = slice_keys(n, splits), s0 = split * chunk, s1 = min(n, s0 + chunk);
-  if (!ALONE && s0 >= s1) return;                       // (the joining launch knows which slices there are)
+  const Slices sl = ALONE ? Slices{n, 1} : slices_of(n, splits);
+  if (!ALONE && split >= sl.count) return;              // (the joining launch knows which slices there are)
+  const int s0 = split * sl.keys, s1 = split == sl.count - 1 ? n : s0 + sl.keys;
 
   __shared__ float sh_m[NW][16], sh_l[NW][16];
   __shared__ float sh_o[NW][16][D + 4];                 // (+ 4: the four quarters of a wave on different banks)
@@ -403,7 +411,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
   const bool idle = a.counts != nullptr && a.counts[r] <= 0;
   const int n = idle ? 0 : held_keys(c, r);
   if (blockIdx.x > 0 && (int)blockIdx.x * JOIN_KEYS >= n) return;
-  const int chunk = slice_keys(n, splits), ns = n > 0 ? (n + chunk - 1) / chunk : 0;
+  const int ns = slices_of(n, splits).count;            // (none where there are no keys)
   const int key = blockIdx.x * JOIN_KEYS + 4 * threadIdx.x;
   const float* sp = ws.scores + (size_t)(r * c.Hkv + kh) * G * ws.ld + min(key, max(0, ws.ld - 4));
   f32x4 s[HB];
@@ -1172,11 +1180,23 @@ bool attend_alone(const BoundedCache& c, int Hq) {
   const int G = Hq / c.Hkv;
   return c.cap <= 512 && c.cap * ((G + 15) / 16) <= 1024 && ((c.cap + 31) & ~31) * G <= ALONE_SCORES;
 }
-// Slices of a row's keys: four workgroups a CU, for long caches two: 32 rows of up to 2048 keys 44.0 us with four, 47.4 with two, 46.8 with eight; 4 of 32761 keys 120, 117, 126.
+// Slices of a row's keys, of u times 128: so many workgroups that they fill two rounds of two a CU (rows are of unequal lengths; long caches, whose slices are, one round) and leave little of
+// the last round empty.  us, 1 / 2 / 3 units a slice: 32 rows of 520 float32 keys, 40 / 8 heads, 37.5 / 44.4 / 37.4; 8 of 2815 46.3 / 45.3 / 43.5; 8 of 1025 24.8 / 27.8 (21.4 without a slice for the last key); 4 of 32761 float16 keys in 16 /
+// 32 / 64 slices 117 / 120 / 126; 32 of 0 to 2048 in 2 / 4 / 8 47.4 / 44.0 / 46.8.
 int attend_splits(const BoundedCache& c, int Hq, int ncu) {
-  const int tiles = c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16), wgs = c.cap >= 16384 ? 2 : 4;
-  return std::max(1, std::min({MAX_SPLITS, (wgs * ncu + tiles - 1) / tiles, (c.cap + 127) / 128}));
+  const int64_t tiles = (int64_t)c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16), units = std::max(1, (c.cap - 32 + 127) / 128), slots = 2 * ncu;
+  const int64_t rounds = c.cap >= 16384 ? 1 : 2, least = (units + MAX_SPLITS - 1) / MAX_SPLITS;
+  const int64_t u0 = std::max(least, (tiles * units + slots * rounds / 2) / (slots * rounds)), from = u0 <= 4 ? least : std::max(least, u0 - 2), to = u0 <= 4 ? 2 * u0 + 2 : u0 + 2;
+  int64_t best = 1, best_off = 0;
+  double best_fill = 0;
+  for (int64_t u = std::min(from, units); u <= std::min(to, units); ++u) {
+    const int64_t s = (units + u - 1) / u, n = (tiles * s + slots - 1) / slots, off = std::abs(n - rounds);
+    const double fill = (double)(tiles * s) / (double)(n * slots);
+    if (fill > 1.05 * best_fill || (fill > 0.95 * best_fill && off <= best_off)) { best = s; best_off = off; best_fill = std::max(fill, best_fill); }
+  }
+  return (int)best;
 }
+
 // All queries of a KV head in one workgroup: where there are few of them, before few keys or in rows and heads enough to fill the chip.  us, alone / in units: 30 queries of 30 keys 7.3 /
 // 12.3, 32 of 256 15.2 / 17.6, 32 of 400 23.3 / 17.3; float32 16 of 100 16.8 / 17.8, of 200 26.1 / 21.8; 64 rows of 8 heads, 32 queries, 400 keys 36 / 61, 4000 keys 294 / 407, float32 16 of 400 84 / 153;
 // 256 rows and heads of 1000 keys 53 / 58; 200 of 300 keys, 3 queries, 18 / 52.
