@@ -160,7 +160,7 @@ int mi_op_sample(float* logits, int B, int V, float temperature, float top_p, co
  * order, and after an eviction slots are in no order of position.
  *
  * These calls enqueue on `stream` (a hipStream_t of the current device, NULL: its null stream) and return; they may be captured into a graph.
- * Calls on one cache follow one another in the order of its stream; ws is the call's own until it has run.  All pointers are device memory,
+ * Calls on one cache follow one another in the order of its stream; ws is the call's own until it has run (a size of 0: none, NULL will do).  All pointers are device memory,
  * arrays are contiguous and aligned to 16 bytes.  What lies in `len`, `next`, `counts` and the block table is read on the device and cannot be refused: a
  * length outside [0, cap] counts as the nearer end, a table entry outside [0, n_blocks) names no block: its keys take no part in attention, and nothing is
  * written for them.  Slots behind a row's length keep what they hold.  The attention of a prompt itself: mi_op_attention_prefill on the same arrays, its

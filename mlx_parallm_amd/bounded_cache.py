@@ -13,7 +13,7 @@ keys per row and KV head, on the kernels of ``csrc/bounded.hip`` (``mi_op_bounde
         out = cache.attend(q[:, 0])                                    # its attention; adds the weights
         cache.evict(budget, keep_first=4, keep_last=32)
 
-Everything is enqueued on torch's current stream of the cache's device, nothing waits: the lengths stay on the device, and the calls can be
+``capacity`` holds the prompt, or the budget and what comes between two evictions.  Everything is enqueued on torch's current stream of the cache's device, nothing waits: the lengths stay on the device, and the calls can be
 captured into a HIP graph.  There are no gradients and no CPU fallback.
 """
 from __future__ import annotations
