@@ -207,7 +207,8 @@ int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int 
 
 /* At most `budget` keys stay in every row: for each KV head those at positions below keep_first or from next - keep_last on before all others, then the more
  * weighted (NaN: as -inf), equal ones by the lower slot.  What stays behind slot `budget` moves into the holes in front of it, the i-th into the
- * i-th, with its position and weight; len becomes min(len, budget). */
+ * i-th, with its position and weight; len becomes min(len, budget).  A slot in a block that is none counts in len, but has no key: in front of `budget` it stays
+ * as it is, behind it it leaves, protected or not, and the best of the other keys take the other slots in front of `budget`. */
 uint64_t mi_op_bounded_evict_ws(const mi_op_bounded_cache* c, int budget);
 int mi_op_bounded_evict(const mi_op_bounded_cache* c, int budget, int keep_first, int keep_last, void* ws, uint64_t ws_bytes, void* stream);
 

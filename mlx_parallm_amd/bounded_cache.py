@@ -152,7 +152,8 @@ class BoundedKVCache:
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_last: int = 0) -> None:
         """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last`` before all
-        others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it."""
+        others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it.
+        Slots in blocks that the table does not name have no key: in front of `budget` they stay as they are and count in it, behind it they leave."""
         n = self._lib.mi_op_bounded_evict_ws(self._ref, budget)
         ws = self._workspace(n)
         self._call(self._lib.mi_op_bounded_evict, self._ref, budget, keep_first, keep_last, _ptr(ws), n)

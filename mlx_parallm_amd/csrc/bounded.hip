@@ -928,7 +928,8 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 // 256 bytes); 256 of 1025 down to 1024, in one launch: 8.5.
 struct EvictWs { int32_t* counts; int2* moves; uint32_t* ranks; int most; };      // [row][KV head]; [row][KV head][most] (from, to); [row][KV head][cap]
 
-// Where more keys are protected than the budget holds, they alone are ranked (`crowded`).
+// Where more keys are protected than the budget holds, they alone are ranked (`crowded`).  A slot in a block that is none has no key: in front of `budget` it stays as it is (no hole, as nothing can be
+// written there), behind it it leaves.  Every other slot in front of `budget` holds a key, so there are always enough of them for what is left of the budget, and no move begins or ends in such a block.
 constexpr uint32_t RANK_STAYS = 0xffffffffu, RANK_LEAVES = 0;
 __device__ __forceinline__ uint32_t rank_of(float w, int pos, int first, int recent_from, bool crowded) {
   if ((pos < first || pos >= recent_from) != crowded) return crowded ? RANK_LEAVES : RANK_STAYS;
@@ -952,7 +953,7 @@ __device__ __forceinline__ void move_rows(const BoundedCache& c, int r, int kh, 
     const int2 m = moves[e / row_pieces];
     const int p = (int)(e % row_pieces);
     const int64_t from = row_of_16(c, r, kh, m.x & ~15), to = row_of_16(c, r, kh, m.y & ~15);
-    if (from < 0 || to < 0) continue;
+    if (from < 0 || to < 0) continue;                              // (the selection has seen to that)
     const int64_t a = (from + (m.x & 15)) * row_pieces + p, b = (to + (m.y & 15)) * row_pieces + p;
     ((u32x4*)c.k)[b] = ((const u32x4*)c.k)[a];
     ((u32x4*)c.v)[b] = ((const u32x4*)c.v)[a];
@@ -1004,6 +1005,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   __shared__ int sh_prot[16], sh_bin, sh_above, sh_in;
   bool crowded = false;
   auto rank = [&](int i) -> uint32_t& { return IN_LDS ? lds_ranks[i + (i >> 5)] : ranks[i]; };
+  const int32_t* table = c.btab != nullptr ? c.btab + (size_t)r * c.bt_stride : nullptr;
 
   // ranks, their range, and how many keys stay whatever their weight
   uint32_t lo, hi;
@@ -1012,14 +1014,15 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
     lo = 0xffffffffu; hi = 0; prot = 0;
     for (int i0 = threadIdx.x; i0 < n; i0 += 8 * THREADS) {        // (the loads of eight slots on their way together)
       float w[8];
-      int32_t p[8];
+      int32_t p[8], block[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { const int i = min(i0 + j * THREADS, n - 1); w[j] = wp[i]; p[j] = pp[i]; }
+      for (int j = 0; j < 8; ++j) { const int i = min(i0 + j * THREADS, n - 1); w[j] = wp[i]; p[j] = pp[i]; block[j] = table != nullptr ? table[i >> c.bs_shift] : 0; }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int i = i0 + j * THREADS;
         if (i >= n) continue;
-        const uint32_t k = rank_of(w[j], p[j], keep_first, recent_from, crowded);
+        const bool lost = table != nullptr && (unsigned)block[j] >= (unsigned)c.n_blocks;
+        const uint32_t k = lost ? (i < budget ? RANK_STAYS : RANK_LEAVES) : rank_of(w[j], p[j], keep_first, recent_from, crowded);
         rank(i) = k;
         if (k == RANK_STAYS) ++prot;
         else if (k != RANK_LEAVES) { lo = min(lo, k); hi = max(hi, k); }
@@ -1044,9 +1047,9 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(BoundedCache c, int 
   int need = 0;
   bool found = false;
   if (n - budget <= FEW && !crowded) {                             // few leave: the least weighted alone (always, where it is one key a step; 9.8 -> 6.5 us of selection)
-    int equal = 0, all;
-    for (int i = threadIdx.x; i < n; i += THREADS) equal += rank(i) == lo;
-    block_scan<THREADS>(equal, all, scan);
+    int least = 0, all;
+    for (int i = threadIdx.x; i < n; i += THREADS) least += rank(i) <= lo;         // (and the slots without a key)
+    block_scan<THREADS>(least, all, scan);
     if (n - all <= budget) {
       cut = lo;
       need = budget - (n - all);

@@ -102,19 +102,19 @@ class Model:
         return wt + asked * U * np.abs(self.w)
 
     def evict(self, budget, first=0, last=0, there=None):
+        """Slots that are not there: in front of `budget` they stay as they are, behind it they leave; the other slots in front of it go to the best of the keys that are."""
         for r in range(self.rows):
             n = self.held(r)
             if n <= budget:
                 continue
+            lost = np.zeros(n, bool) if there is None else ~there[r, :n]
             for h in range(self.heads):
                 p, w = self.pos[r, h, :n], self.w[r, h, :n]
                 apart = (p < first) | (p >= self.next[r] - last)
                 order = np.lexsort((np.arange(n), -np.where(np.isnan(w), -np.inf, w), ~apart))
-                stays = np.zeros(n, bool)
-                stays[order[:budget]] = True
+                stays = lost & (np.arange(n) < budget)
+                stays[order[~lost[order]][:budget - stays.sum()]] = True
                 frm, to = np.flatnonzero(stays[budget:]) + budget, np.flatnonzero(~stays[:budget])
                 self.pos[r, h, to], self.w[r, h, to] = self.pos[r, h, frm], self.w[r, h, frm]
-                for f, t in zip(frm, to):
-                    if there is None or (there[r, f] and there[r, t]):
-                        self.k[r, h, t], self.v[r, h, t] = self.k[r, h, f], self.v[r, h, f]
+                self.k[r, h, to], self.v[r, h, to] = self.k[r, h, frm], self.v[r, h, frm]
             self.len[r] = budget
