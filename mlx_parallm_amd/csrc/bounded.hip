@@ -27,6 +27,9 @@ constexpr int MAX_GROUP = 128;          // query heads per KV head
 // one fused operation leaves the rounding of scale * m, 2^5 where a score is 2^30).
 __device__ __forceinline__ float weight_of(float s, float m, float sc) { return __builtin_amdgcn_exp2f((s - m) * sc); }
 
+// The same for a sum whose maximum is m, of sums whose largest maximum is M: never quite zero, so that what is infinite in it stays infinite.
+__device__ __forceinline__ float share_of(float m, float M, float sc) { return fmaxf(weight_of(m, M, sc), 1.401298464e-45f); }
+
 __device__ __forceinline__ int held_keys(const BoundedCache& c, int r) { return min(max(c.len[r], 0), c.cap); }
 
 // Places of 16 keys that begin at a multiple of 16: one block of a paged cache (blocks are powers of two from 16 on).  The index of the first
@@ -220,9 +223,20 @@ __device__ __forceinline__ u32x4 column(const Raw<E * 2> (&v)[8], int j) {      
   return u32x4{o[0], o[1], o[2], o[3]};
 }
 
+// An infinite value is infinite at any weight, but its product with a 16-bit weight's second term (zero, or of the other sign) is NaN, or with a weight that is zero in its type.  Where there are any
+// (`INFINITE`: the sums of a first walk over the keys were not finite) they enter the products apart from the others, with one for a weight (zero for a score of -inf, which has none: bit 4 t + i of `some`).
+// float32 has the one product: infinite, or NaN where the weight is zero in float32.
+template <typename T>
+__device__ __forceinline__ u32x4 infinite_ones(u32x4 a) {
+  constexpr uint32_t INF = std::is_same_v<T, bf16> ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] &= ((a[i] & 0x7fffu) == INF ? 0xffffu : 0) | ((a[i] & 0x7fff0000u) == INF << 16 ? 0xffff0000u : 0);
+  return a;
+}
+
 // O^T += V^T P^T for the keys of a tile: v[4 t + i] is this lane's E elements of key 16 t + 4 q + i, p[t][i] that key's weight
-template <typename T, int E>
-__device__ __forceinline__ void add_values(const Raw<E * 2> (&v)[8], const float (&p)[2][4], f32x4 (&o)[E]) {
+template <typename T, int E, bool INFINITE>
+__device__ __forceinline__ void add_values(const Raw<E * 2> (&v)[8], const float (&p)[2][4], f32x4 (&o)[E], uint32_t some) {
   uint32_t hi[4], lo[4];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -230,9 +244,21 @@ __device__ __forceinline__ void add_values(const Raw<E * 2> (&v)[8], const float
     pack2_split<T>(p[t][2], p[t][3], hi[2 * t + 1], lo[2 * t + 1]);
   }
   const u32x4 ph{hi[0], hi[1], hi[2], hi[3]}, pl{lo[0], lo[1], lo[2], lo[3]};
+  u32x4 ones{0, 0, 0, 0};
+  if constexpr (INFINITE) {
+    constexpr uint32_t ONE = std::is_same_v<T, bf16> ? 0x3f80u : 0x3c00u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i / 2] |= some >> i & 1 ? ONE << 16 * (i & 1) : 0;
+  }
 #pragma unroll
   for (int j = 0; j < E; ++j) {
-    const u32x4 a = column<E>(v, j);
+    u32x4 a = column<E>(v, j);
+    if constexpr (INFINITE) {
+      const u32x4 b = infinite_ones<T>(a);
+      a ^= b;
+      o[j] = mfma16<T>(b, ones, o[j]);
+      __builtin_amdgcn_sched_barrier(0);               // (one after the other: this rare way asks for no more registers than the other)
+    }
     o[j] = mfma16<T>(a, ph, o[j]);
     o[j] = mfma16<T>(a, pl, o[j]);
   }
@@ -266,8 +292,15 @@ struct AttendWs {
   float* scores; float* stats; float* part; int ld;
 };
 
+// Waves a SIMD: as many as the first walk over the keys needs (the second, over infinite values, would ask for more registers where it is let).
 template <typename T, int E, bool ALONE>
-__global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
+constexpr int attend_waves() {
+  if (ALONE) return E > 8 ? 1 : 2;
+  return sizeof(T) == 4 ? (E <= 4 ? 4 : E <= 6 ? 3 : E <= 12 ? 2 : 1) : (E == 1 ? 6 : E == 2 ? 5 : E <= 6 ? 4 : E <= 8 ? 3 : E <= 12 ? 2 : 1);
+}
+
+template <typename T, int E, bool ALONE>
+__global__ __launch_bounds__(256, (attend_waves<T, E, ALONE>())) void attend_kernel(BoundedCache c, BoundedAttend a, AttendWs ws, int splits) {
   constexpr int D = 16 * E, NW = 4;
   constexpr int SUB = sizeof(T) == 4 && E > 8 ? 1 : 2, KT = 16 * SUB;      // (float32 heads of 192 and 256: registers for 16 keys)
   const int G = a.Hq / c.Hkv, split = blockIdx.x, kh = blockIdx.y % c.Hkv, r = blockIdx.y / c.Hkv;
@@ -290,63 +323,81 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
     Frag<T, D> q, k[SUB];
     Raw<E * (int)sizeof(T)> v[4 * SUB];
     q.load((const T*)a.q + ((size_t)r * a.Hq + kh * G + h0 + ln) * D, qd, ln < heads);
-    float m = LOWEST, l = 0.f;
+    float m, l;
     f32x4 o[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float* sc_out = ws.scores + ((size_t)(r * c.Hkv + kh) * G + h0 + ln) * ws.ld;      // (in slices)
     const int sh_at = (h0 + ln) * ws.ld;                                                // (alone)
 
-    for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
-      bool there[SUB];
+    auto walk = [&](auto infinite) {                                     // true_type: 16-bit values that are infinite among them
+      constexpr bool INFINITE = decltype(infinite)::value;
+      m = LOWEST; l = 0.f;
 #pragma unroll
-      for (int t = 0; t < SUB; ++t) {
-        const int key = __builtin_amdgcn_readfirstlane(base + 16 * t);
-        const int64_t at = key < s1 ? row_of_16(c, r, kh, key) : -1;
-        there[t] = at >= 0;
-        const int last = there[t] ? min(15, s1 - 1 - key) : 0;           // (a clamped address: its scores are masked, its values cleared)
-        const T* kp = (const T*)c.k + (there[t] ? at : 0) * D;
-        const T* vp = (const T*)c.v + (there[t] ? at : 0) * D;
-        k[t].load(kp + (int64_t)min(ln, last) * D, qd);
+      for (int j = 0; j < E; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int base = s0 + wave * KT; base < s1; base += NW * KT) {
+        bool there[SUB];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * t + i] = load_bits<E * (int)sizeof(T)>(vp + (int64_t)min(4 * qd + i, last) * D + ln * E);
-      }
-      float p[SUB][4];
-      float top = -INFINITY;
+        for (int t = 0; t < SUB; ++t) {
+          const int key = __builtin_amdgcn_readfirstlane(base + 16 * t);
+          const int64_t at = key < s1 ? row_of_16(c, r, kh, key) : -1;
+          there[t] = at >= 0;
+          const int last = there[t] ? min(15, s1 - 1 - key) : 0;           // (a clamped address: its scores are masked, its values cleared)
+          const T* kp = (const T*)c.k + (there[t] ? at : 0) * D;
+          const T* vp = (const T*)c.v + (there[t] ? at : 0) * D;
+          k[t].load(kp + (int64_t)min(ln, last) * D, qd);
 #pragma unroll
-      for (int t = 0; t < SUB; ++t) {
-        f32x4 s = dot16(k[t], q);
-        const int key = base + 16 * t + 4 * qd;
-        if (base + KT > s1 || !there[t]) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (key + i >= s1 || !there[t]) {
-              s[i] = -INFINITY;
-#pragma unroll
-              for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
-            }
+          for (int i = 0; i < 4; ++i) v[4 * t + i] = load_bits<E * (int)sizeof(T)>(vp + (int64_t)min(4 * qd + i, last) * D + ln * E);
         }
-        if (ln < heads && key < s1) {                                    // (`ld` reaches to the tile's end)
-          if constexpr (ALONE) *(f32x4*)&all_s[sh_at + key] = s;
-          else *(f32x4*)(sc_out + key) = s;
+        float p[SUB][4];
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < SUB; ++t) {
+          f32x4 s = dot16(k[t], q);
+          const int key = base + 16 * t + 4 * qd;
+          if (base + KT > s1 || !there[t]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (key + i >= s1 || !there[t]) {
+                s[i] = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < (int)(sizeof(v[0].w) / 4); ++w) v[4 * t + i].w[w] = 0;
+              }
+          }
+          if (ln < heads && key < s1) {                                    // (`ld` reaches to the tile's end)
+            if constexpr (ALONE) *(f32x4*)&all_s[sh_at + key] = s;
+            else *(f32x4*)(sc_out + key) = s;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
+        }
+        if (__any(top > m + step)) {
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float now = fmaxf(m, top), f = INFINITE ? share_of(m, now, sc) : weight_of(m, now, sc);
+          m = now; l *= f;
+#pragma unroll
+          for (int j = 0; j < E; ++j) o[j] *= f;
+        }
+        uint32_t some = 0;
+        if constexpr (INFINITE) {
+#pragma unroll
+          for (int i = 0; i < 4 * SUB; ++i) some |= p[i / 4][i % 4] > -INFINITY ? 1u << i : 0;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { p[t][i] = s[i]; top = fmaxf(top, s[i]); }
+        for (int t = 0; t < SUB; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
+        if constexpr (sizeof(T) == 2) add_values<T, E, INFINITE>(v, p, o, some);
+        else add_values<T, E, SUB>(v, p, o);
       }
-      if (__any(top > m + step)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float now = fmaxf(m, top), f = weight_of(m, now, sc);
-        m = now; l *= f;
+    };
+    walk(std::false_type{});
+    if constexpr (sizeof(T) == 2) {
+      f32x4 odd{0.f, 0.f, 0.f, 0.f};                                     // (NaN once anything is not finite)
 #pragma unroll
-        for (int j = 0; j < E; ++j) o[j] *= f;
-      }
+      for (int j = 0; j < E; ++j)
 #pragma unroll
-      for (int t = 0; t < SUB; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
-      if constexpr (sizeof(T) == 2) add_values<T, E>(v, p, o);
-      else add_values<T, E, SUB>(v, p, o);
+        for (int i = 0; i < 4; ++i) odd[i] = fmaf(o[j][i], 0.f, odd[i]);
+      if (__any((odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f)) walk(std::true_type{});
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -363,7 +414,7 @@ __global__ __launch_bounds__(256, E > 8 ? 1 : 2) void attend_kernel(BoundedCache
       M = fmaxf(fmaxf(sh_m[0][h], sh_m[1][h]), fmaxf(sh_m[2][h], sh_m[3][h]));
       L = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) { f[w] = weight_of(sh_m[w][h], M, sc); L = fmaf(sh_l[w][h], f[w], L); }
+      for (int w = 0; w < NW; ++w) { f[w] = share_of(sh_m[w][h], M, sc); L = fmaf(sh_l[w][h], f[w], L); }
     };
     const size_t slice = ((size_t)(r * c.Hkv + kh) * splits + split) * G + h0;
     for (int e = threadIdx.x; e < heads * D; e += 256) {
@@ -471,7 +522,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
     for (int i0 = 0; i0 < ns; i0 += 8) {
       if (e != e0 || i0 > 0) fetch_out(e, i0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], weight_of(om[j], sh_m[h], sc), x) : x;
+      for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], share_of(om[j], sh_m[h], sc), x) : x;
     }
     ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
   }
