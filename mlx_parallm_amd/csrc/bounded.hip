@@ -26,6 +26,7 @@ constexpr int MAX_GROUP = 128;          // query heads per KV head
 // exp(scale * (s - m)) of products s and m <= s's maximum, sc = scale * log2 e.  The difference first: at its maximum a score of any size weighs one (scale * s - scale * m in
 // one fused operation leaves the rounding of scale * m, 2^5 where a score is 2^30).
 __device__ __forceinline__ float weight_of(float s, float m, float sc) { return __builtin_amdgcn_exp2f((s - m) * sc); }
+__device__ __forceinline__ float weight_of(float s, float m, float sc, float up) { return __builtin_amdgcn_exp2f(fmaf(s - m, sc, up)); }      // times 2^up
 
 // The same for a sum whose maximum is m, of sums whose largest maximum is M: never quite zero, so that what is infinite in it stays infinite.
 __device__ __forceinline__ float share_of(float m, float M, float sc) { return fmaxf(weight_of(m, M, sc), 1.401298464e-45f); }
@@ -176,12 +177,18 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // the keys that the same lane multiplies in O^T += V^T P^T, and every rescale is the lane's own.  16-bit: a tile is 32 keys, 16 x 16 x 32
 // products; the slot k = 8 q + 4 t + i of the second product stands for key 16 t + 4 q + i (q = lane >> 4), which is where the first left
 // it.  A lane loads E = D / 16 elements of 8 keys' values -- whole rows across 16 lanes -- and transposes its 8 x E block in registers
-// (v_perm); column n of output tile j is element n E + j.  P goes in as two 16-bit terms (2^-17).  float32: 16 x 16 x 4 products, no
-// transposition.  The largest score so far is taken in when a new one exceeds it by 2^8, not at every tile.
+// (v_perm); column n of output tile j is element n E + j.  P goes in as two 16-bit terms, off by 2^-17 (bfloat16), 2^-22 (float16) of it at most.  float32: 16 x 16 x 4 products, no
+// transposition.  The largest score so far is taken in when a new one exceeds it by 2^8 (float16: 2), not at every tile.
+// float16 ends at 2^-24, and many keys far below the largest may be all there is where that one's value is small.  So P is 2^13 there, at most 2^15, where the score is the largest so far, and a tile whose
+// largest is 2^11 below is raised until it is not, the sums with it: by a power of two, which rounds nothing, and down again behind it.  A weight is off by 2^-27 of the largest of its tile of 32 keys at most.
 // What a key weighs needs the final maximum and sum of every head, so the products are kept (4 bytes a head and key, 3 % of 16-bit keys and values at 4 heads) and read by whoever has
 // them: the workgroup itself where it is alone (`ALONE`), else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
 // Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
 // launches' heads; 8 rows of 1025 float32 keys, 68 MB, 19.4 + 4.2: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
+
+// P is 2^UP where the score is the largest, in the sums of weights and values alike.
+template <typename T>
+constexpr float UP = std::is_same_v<T, f16> ? 13.f : 0.f;
 
 // A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
 template <typename T, int D>
@@ -296,7 +303,8 @@ struct AttendWs {
 template <typename T, int E, bool ALONE>
 constexpr int attend_waves() {
   if (ALONE) return E > 8 ? 1 : 2;
-  return sizeof(T) == 4 ? (E <= 4 ? 4 : E <= 6 ? 3 : E <= 12 ? 2 : 1) : (E == 1 ? 6 : E == 2 ? 5 : E <= 6 ? 4 : E <= 8 ? 3 : E <= 12 ? 2 : 1);
+  if (sizeof(T) == 4) return E <= 4 ? 4 : E <= 6 ? 3 : E <= 12 ? 2 : 1;
+  return std::is_same_v<T, f16> ? (E == 1 ? 5 : E <= 4 ? 4 : E <= 8 ? 3 : E <= 12 ? 2 : 1) : (E == 1 ? 6 : E == 2 ? 5 : E <= 6 ? 4 : E <= 8 ? 3 : E <= 12 ? 2 : 1);
 }
 
 template <typename T, int E, bool ALONE>
@@ -316,7 +324,8 @@ __global__ __launch_bounds__(256, (attend_waves<T, E, ALONE>())) void attend_ker
   __shared__ float all_m[ALONE ? MAX_GROUP : 1], all_r[ALONE ? MAX_GROUP : 1];
   __shared__ __align__(16) float all_s[ALONE ? ALONE_SCORES : 4];
   const float sc = a.scale * LOG2E;
-  const float step = 8.f / sc;                          // 2^8
+  constexpr bool F16 = std::is_same_v<T, f16>;
+  const float step = (F16 ? 1.f : 8.f) / sc;            // 2, 2^8
   for (int h0 = blockIdx.z * 16; h0 < G; h0 += 16 * gridDim.z) {
     const int heads = min(16, G - h0);
     T* out = (T*)a.out + ((size_t)r * a.Hq + kh * G + h0) * D;
@@ -377,6 +386,20 @@ __global__ __launch_bounds__(256, (attend_waves<T, E, ALONE>())) void attend_ker
 #pragma unroll
           for (int j = 0; j < E; ++j) o[j] *= f;
         }
+        float up = UP<T>, down = 1.f;
+        bool raised = false;
+        if constexpr (F16) {
+          raised = __any(top < m - 11.f / sc);
+          if (raised) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float by = fminf(fmaxf(floorf((m - top) * sc), 0.f), 60.f);      // (sums are below 2^61)
+            up += by;
+            down = ldexpf(1.f, -(int)by);
+#pragma unroll
+            for (int j = 0; j < E; ++j) o[j] *= ldexpf(1.f, (int)by);
+          }
+        }
         uint32_t some = 0;
         if constexpr (INFINITE) {
 #pragma unroll
@@ -385,9 +408,16 @@ __global__ __launch_bounds__(256, (attend_waves<T, E, ALONE>())) void attend_ker
 #pragma unroll
         for (int t = 0; t < SUB; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { p[t][i] = weight_of(p[t][i], m, sc); l += p[t][i]; }
+          for (int i = 0; i < 4; ++i) {
+            p[t][i] = weight_of(p[t][i], m, sc, up);
+            l = F16 ? fmaf(p[t][i], down, l) : l + p[t][i];
+          }
         if constexpr (sizeof(T) == 2) add_values<T, E, INFINITE>(v, p, o, some);
         else add_values<T, E, SUB>(v, p, o);
+        if (raised) {
+#pragma unroll
+          for (int j = 0; j < E; ++j) o[j] *= down;
+        }
       }
     };
     walk(std::false_type{});
@@ -445,7 +475,7 @@ __global__ __launch_bounds__(256, (attend_waves<T, E, ALONE>())) void attend_ker
     for (int key = threadIdx.x; key < n; key += 256) {
       const float w = wp[key];
       float x = 0.f;
-      for (int h = 0; h < G; ++h) x = fmaf(weight_of(all_s[h * ws.ld + key], all_m[h], sc), all_r[h], x);
+      for (int h = 0; h < G; ++h) x = fmaf(weight_of(all_s[h * ws.ld + key], all_m[h], sc, UP<T>), all_r[h], x);
       wp[key] = w + x;
     }
   }
@@ -510,7 +540,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
       for (int j = 0; j < HB; ++j)
         if (h0 + j < G)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fmaf(weight_of(s[j][i], sh_m[h0 + j], sc), sh_r[h0 + j], x[i]);
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(weight_of(s[j][i], sh_m[h0 + j], sc, UP<T>), sh_r[h0 + j], x[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)

@@ -1,10 +1,11 @@
-"""Values at the ends of their types in the attention of a cache of fixed size."""
+"""Values at the ends of their types, and weights far below the largest, in the attention of a cache of fixed size."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 import torch
 
+from tests.bounded_model import HALF, TINY
 from tests.test_gpu_bounded import DT, Setup, f64, within
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +67,62 @@ def test_infinite_values_of_keys_that_weigh_little(n, first, dtype):
     q = torch.zeros(1, 2, D, dtype=DT[dtype])
     q[..., 0] = 8.0
     assert (attend_with_infinities(s, 2, q)[0, :, 1] == -INF).all()
+
+
+# ---- float16: weights far below the largest
+
+def exact(q, k, v):
+    s = k @ q / len(q) ** 0.5
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    return p, p @ v
+
+
+def tolerance(q, k, v, p, o):
+    """What 32 bits leave in scores and sums (as the model has it: D products and sums, the exponent to base 2 twice; a sum of at most 256 terms in a row: 24 keys' worth of a wave's three tiles in a lane and
+    96 in a matrix instruction's, twice for the two terms, then 4 waves and up to 64 slices); P as two float16 numbers, half a step of half a step of each
+    or half of float16's smallest number, of which the largest weight of the 32 keys of a tile is at least 2^26; the output's own rounding."""
+    n, u = len(p), 2.0 ** -24
+    off = (len(q) + 4) * u * float((np.abs(k) @ np.abs(q)).max()) / len(q) ** 0.5 + 4 * u * (1 + float(np.abs(k @ q).max()) / len(q) ** 0.5)
+    tile = np.repeat(np.maximum.reduceat(p, np.arange(0, n, 32)), 32)[:n]
+    t = (2 * off + (2 * min(n, 256) + 16) * u + 2 * HALF["float16"] ** 2) * (p @ np.abs(v)) + 2.0 ** -27 * (tile @ np.abs(v))
+    return t + (np.abs(o) + t) * HALF["float16"] + TINY["float16"]
+
+
+@pytest.mark.parametrize("gap", [8.0, 13.0, 16.0, 18.0])
+@pytest.mark.parametrize("n,at", [(50, 0), (500, 0), (2000, 1999), (20000, 0), (20000, 11111)])
+def test_weights_far_below_the_largest(n, at, gap):
+    """One key takes nearly all of the weight and its value is nothing: the output is what the others hold, each of them `gap` nats below."""
+    D, Hq = 64, 4
+    s = Setup(n + at, 1, 1, D, n, [n], "float16")
+    k = torch.randn((n, D), generator=s.g) * 0.02
+    k[:, 0], k[at, 0] = 0, gap
+    v = 1 + torch.rand((n, D), generator=s.g)
+    v[at] = 0
+    s.cache.keys[0, 0], s.cache.values[0, 0] = k.half().cuda(), v.half().cuda()
+    q = s.randn(1, Hq, D)
+    q[..., 0] = 8.0                                       # 8 gap / sqrt(64)
+    out = f64(s.cache.attend(q.cuda()))[0]
+    kk, vv = f64(s.cache.keys)[0, 0], f64(s.cache.values)[0, 0]
+    for h in range(Hq):
+        p, o = exact(f64(q)[0, h], kk, vv)
+        within(out[h], o, tolerance(f64(q)[0, h], kk, vv, p, o))
+
+
+@pytest.mark.parametrize("n", [300, 5000])
+def test_widely_spread_scores(n):
+    """Scores over 30 nats, values that grow as their weights fall, to float16's largest."""
+    D, Hq = 64, 5
+    s = Setup(n, 2, 1, D, n, [n, n - 1], "float16")
+    k = torch.zeros((2, n, D))
+    k[..., 0] = -30 * torch.rand((2, n), generator=s.g)
+    v = torch.randn((2, n, D), generator=s.g) * torch.exp(-k[..., :1]).clamp_max(20000.0)
+    s.cache.keys[:, 0], s.cache.values[:, 0] = k.half().cuda(), v.clamp(-65504, 65504).half().cuda()
+    q = torch.zeros(2, Hq, D, dtype=torch.float16)
+    q[..., 0] = 8.0
+    out = f64(s.cache.attend(q.cuda()))
+    for r in range(2):
+        kk, vv = f64(s.cache.keys)[r, 0, :n - r], f64(s.cache.values)[r, 0, :n - r]
+        for h in range(Hq):
+            p, o = exact(f64(q)[r, h], kk, vv)
+            within(out[r, h], o, tolerance(f64(q)[r, h], kk, vv, p, o))
