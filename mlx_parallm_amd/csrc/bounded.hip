@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 #pragma unroll
       for (int j = 0; j < 8; ++j) x = i0 + j < ns ? fmaf(o[j], share_of(om[j], sh_m[h], sc), x) : x;
     }
-    ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(x * sh_r[h]);
+    ((T*)a.out)[((size_t)r * a.Hq + kh * G) * D + e] = (T)(sh_r[h] != 0.f ? x * sh_r[h] : 0.f);      // (nothing to see: whatever the values are)
   }
 }
 

@@ -126,3 +126,20 @@ def test_widely_spread_scores(n):
         for h in range(Hq):
             p, o = exact(f64(q)[r, h], kk, vv)
             within(out[r, h], o, tolerance(f64(q)[r, h], kk, vv, p, o))
+
+
+# ---- nothing to see
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("n", [40, 1500])
+def test_scores_of_minus_infinity_alone(n, dtype):
+    """Nothing to see: zeros, whatever the values hold."""
+    s = Setup(n, 2, 1, 64, n, [n, n], dtype)
+    c = s.cache
+    c.keys[0] = -INF
+    c.values[0] = INF
+    before = c.weights.clone()
+    q = torch.rand((2, 4, 64), generator=s.g).add_(0.5).to(DT[dtype]).cuda()
+    out = c.attend(q)
+    assert (out[0] == 0).all() and torch.equal(c.weights[0], before[0])
+    assert torch.isfinite(out[1]).all() and not torch.equal(c.weights[1], before[1])
