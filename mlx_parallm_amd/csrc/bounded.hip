@@ -186,9 +186,10 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
 // launches' heads; 8 rows of 1025 float32 keys, 68 MB, 19.4 + 4.2: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
 
-// P is 2^UP where the score is the largest, in the sums of weights and values alike.
+// P is 2^UP where the score is the largest, in the sums of weights and values alike.  Below one where values reach to the end of float32, whose sums then stay inside it: 2^16 of them at 2^8, the most that P
+// goes beyond it.
 template <typename T>
-constexpr float UP = std::is_same_v<T, f16> ? 13.f : 0.f;
+constexpr float UP = std::is_same_v<T, f16> ? 13.f : -24.f;
 
 // A row of D elements as an operand of the first product: 16-byte pieces, piece c of a lane from element (4 c + q) 16 bytes on.
 template <typename T, int D>

@@ -143,3 +143,25 @@ def test_scores_of_minus_infinity_alone(n, dtype):
     out = c.attend(q)
     assert (out[0] == 0).all() and torch.equal(c.weights[0], before[0])
     assert torch.isfinite(out[1]).all() and not torch.equal(c.weights[1], before[1])
+
+
+# ---- values near the largest of their type
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("n", [40, 700])
+def test_values_of_the_types_size(n, dtype):
+    """An average of numbers near the type's largest is no larger than they are, in whatever order the scores rise."""
+    D = 64
+    s = Setup(n, 2, 1, D, n, [n, n], dtype)
+    c = s.cache
+    k = torch.zeros((2, n, D))
+    k[0, :, 0], k[1, :, 0] = torch.linspace(-4, 4, n), 0.5
+    c.keys[:, 0] = k.to(DT[dtype]).cuda()
+    big = torch.finfo(DT[dtype]).max * 0.9
+    sign = torch.where(torch.rand((2, 1, n, D), generator=s.g) < 0.7, 1.0, -1.0)
+    sign[..., 0] = 1
+    c.values.copy_((sign.double() * big).to(DT[dtype]))
+    q = torch.zeros(2, 4, D, dtype=DT[dtype])
+    q[..., 0] = 8.0
+    want = attend_with_infinities(s, 4, q)
+    assert np.isfinite(want).all()
