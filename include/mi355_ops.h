@@ -178,7 +178,8 @@ typedef struct mi_op_bounded_cache {
 
 /* New tokens: queries and keys are normed per head (x / sqrt(mean x^2 + eps) * w; no norm where the weights are NULL), rotated by the angles of their
  * positions (pairs i, i + D / 2), keys and values go to the slots from len on, with their positions and weight 0; len and next move on.
- * A row takes min(counts, L, cap - len, max_pos - next) tokens (counts NULL: L), its first ones; queries of the others are zeros. */
+ * A row takes min(counts, L, cap - len, max_pos - next) tokens (counts NULL: L), its first ones; queries of the others are zeros.  `taken` says how many: the counts that
+ * the calls below want for these queries (with the counts that were asked for, a row that was cut short would be taken for one that was not). */
 typedef struct mi_op_bounded_tokens {
   const void* qkv;                   /* token t of row r: [(Hq + 2 Hkv) * D] at r * ld_row + t * ld_token elements (strides: whole 16 bytes) */
   int64_t ld_row, ld_token;
@@ -189,12 +190,13 @@ typedef struct mi_op_bounded_tokens {
   int32_t max_pos;
   const float* cos_tab; const float* sin_tab;      /* [max_pos][D / 2] (mi_op_rope_tables) */
   void* q_out;                       /* [rows][L][Hq][D] */
+  int32_t* taken;                    /* [rows] or NULL: how many tokens the row took (may be `counts`) */
 } mi_op_bounded_tokens;
 int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_tokens* t, void* stream);
 
 /* Attention of one query per row and head, q and out [rows][Hq][D], over all keys that the row holds (its own, just appended, among them); the weight that
  * every key receives, summed over the query heads of its KV head, is added to `weight`.  A row with nothing to see (no keys, or scores of -inf
- * alone), or with counts[row] <= 0, gives zeros.
+ * alone), or with counts[row] <= 0 (it took no token), gives zeros, and its keys receive nothing.
  * Hq / Hkv <= 128, Hq <= 8192 (all of these calls), scale > 0.  ws_bytes: mi_op_bounded_attend_ws, which needs no pointer. */
 uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq);
 int mi_op_bounded_attend(const mi_op_bounded_cache* c, const void* q, int Hq, const int32_t* counts, float scale, void* out, void* ws, uint64_t ws_bytes, void* stream);

@@ -27,7 +27,7 @@ MI_GATE_NONE, MI_GATE_SILU, MI_GATE_SIGMOID, MI_GATE_SIGMOID_HEAD = 0, 1, 2, 3
 MI_QK_NORM_FIRST, MI_QK_NORM_LAST = 0, 1
 MI_ROT_HALVES, MI_ROT_PAIRS = 0, 1
 MI_MAX_TOP_LOGPROBS = 20
-MI_ABI_VERSION = 6
+MI_ABI_VERSION = 7
 WK = {"f32": 0, "bf16": 1, "f16": 2, "q4_f32": 3, "q4_bf16": 4, "q4_f16": 5, "q8_f32": 6, "q8_bf16": 7, "q8_f16": 8}
 RND_NONE, RND_BF16, RND_F16 = 0, 1, 2
 PRO_NONE, PRO_NORM = 0, 1
@@ -106,7 +106,7 @@ class OpBoundedCache(C.Structure):
 class OpBoundedTokens(C.Structure):
     _fields_ = [("qkv", C.c_void_p), ("ld_row", C.c_int64), ("ld_token", C.c_int64), ("L", C.c_int32), ("Hq", C.c_int32), ("counts", C.c_void_p),
                 ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("eps", C.c_float), ("max_pos", C.c_int32), ("cos_tab", C.c_void_p),
-                ("sin_tab", C.c_void_p), ("q_out", C.c_void_p)]
+                ("sin_tab", C.c_void_p), ("q_out", C.c_void_p), ("taken", C.c_void_p)]
 
 
 # name -> (restype, argtypes); every symbol the two headers declare

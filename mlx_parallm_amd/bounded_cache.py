@@ -6,14 +6,15 @@ keys per row and KV head, on the kernels of ``csrc/bounded.hip`` (``mi_op_bounde
     cache = BoundedKVCache.create(rows, kv_heads, head_dim, capacity, dtype="bfloat16")
     q = cache.append(qkv, heads, cos, sin, counts=prompt_lengths)      # norms, rotation, append; [rows, L, heads, head_dim]
     ...                                                                # the prompt's attention (mi_op_attention_prefill reads the same arrays)
-    cache.weigh(q, counts=prompt_lengths)                              # what weight the prompt's queries give every key
+    cache.weigh(q, counts=cache.taken)                                 # what weight the prompt's queries give every key
     cache.evict(budget, keep_first=4, keep_last=32)
     while generating:
         q = cache.append(qkv, heads, cos, sin)                         # one token a row
-        out = cache.attend(q[:, 0])                                    # its attention; adds the weights
+        out = cache.attend(q[:, 0], counts=cache.taken)                # its attention; adds the weights
         cache.evict(budget, keep_first=4, keep_last=32)
 
-``capacity`` holds the prompt, or the budget and what comes between two evictions.  Everything is enqueued on torch's current stream of the cache's device, nothing waits: the lengths stay on the device, and the calls can be
+``capacity`` holds the prompt, or the budget and what comes between two evictions.  A row that is full, or at the end of the angle tables, takes fewer tokens than it is given: ``taken`` says how many the
+last append took, and with it as ``counts`` the others' queries (zeros) ask for nothing.  Everything is enqueued on torch's current stream of the cache's device, nothing waits: the lengths stay on the device, and the calls can be
 captured into a HIP graph.  There are no gradients and no CPU fallback.
 """
 from __future__ import annotations
@@ -78,7 +79,7 @@ class BoundedKVCache:
         c.k, c.v, c.btab = keys.data_ptr(), values.data_ptr(), _ptr(block_table)
         c.len, c.next, c.pos, c.weight = lengths.data_ptr(), next_positions.data_ptr(), positions.data_ptr(), weights.data_ptr()
         # copied from the host, which waits: calls may come on any stream from here on (and a cache is not made while a graph is captured)
-        self._tickets = torch.zeros(rows, dtype=torch.int32).to(self.device)
+        self._tickets, self.taken = torch.zeros((2, rows), dtype=torch.int32).to(self.device)
         c.tickets = self._tickets.data_ptr()
         self._c, self._ref, self._lib = c, C.byref(c), L.lib()
 
@@ -104,7 +105,7 @@ class BoundedKVCache:
         """New tokens: ``qkv`` [rows, L, (heads + 2 kv_heads) * head_dim] (any strides of whole 16 bytes over rows and tokens) -> queries
         [rows, L, heads, head_dim], normed (where ``q_norm`` / ``k_norm`` [head_dim] are given) and rotated by ``cos`` / ``sin``
         [positions, head_dim / 2] float32.  ``counts`` [rows] int32: row r takes its first counts[r] tokens, the queries of the others are zeros.  A row
-        takes no more than it has slots and the tables have positions."""
+        takes no more than it has slots and the tables have positions; ``taken`` [rows] int32 holds from now on how many it took."""
         D, f32 = self.head_dim, torch.float32
         self._check(qkv, "qkv", self.dtype)
         rows, tokens, width = qkv.shape if qkv.dim() == 3 else (0, 0, 0)
@@ -121,13 +122,14 @@ class BoundedKVCache:
                     raise ValueError(f"norm weights: [{D}]")
         q = qkv.new_empty((rows, tokens, heads, D))
         a = L.OpBoundedTokens(qkv.data_ptr(), qkv.stride(0), qkv.stride(1), tokens, heads, self._counts(counts), _ptr(q_norm), _ptr(k_norm), eps, cos.shape[0],
-                              cos.data_ptr(), sin.data_ptr(), q.data_ptr())
+                              cos.data_ptr(), sin.data_ptr(), q.data_ptr(), self.taken.data_ptr())
         self._call(self._lib.mi_op_bounded_append, self._ref, C.byref(a))
         return q
 
     def attend(self, q, scale: Optional[float] = None, *, counts=None):
         """Attention of one query per row, ``q`` [rows, heads, head_dim], over all keys that the row holds -> the same shape; adds the weight
-        that every key receives to ``weights``.  scale: 1 / sqrt(head_dim).  Rows without keys, or with counts[r] <= 0: zeros."""
+        that every key receives to ``weights``.  scale: 1 / sqrt(head_dim).  Rows without keys, or with counts[r] <= 0 (``counts=cache.taken``: that
+        took no token): zeros, and no weights."""
         self._check(q, "q", self.dtype)
         if q.dim() != 3 or q.shape[0] != self.rows or q.shape[2] != self.head_dim:
             raise ValueError(f"q: [{self.rows}, heads, {self.head_dim}]")
@@ -141,7 +143,8 @@ class BoundedKVCache:
 
     def weigh(self, q, scale: Optional[float] = None, *, counts=None, last: int = 0) -> None:
         """Adds the attention weights of a prompt's queries to ``weights``: ``q`` [rows, L, heads, head_dim], of which the first counts[r] are
-        those of the row's last counts[r] slots; each sees the slots up to its own.  last > 0: only the last `last` queries ask."""
+        those of the row's last counts[r] slots; each sees the slots up to its own.  Behind an append: ``counts=cache.taken``.  last > 0: only the last
+        `last` queries ask."""
         self._check(q, "q", self.dtype)
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != self.head_dim:
             raise ValueError(f"q: [{self.rows}, tokens, heads, {self.head_dim}]")

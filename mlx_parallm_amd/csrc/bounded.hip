@@ -160,7 +160,11 @@ __global__ __launch_bounds__(STEP ? 1024 : 256) void append_kernel(BoundedCache 
   }
   if constexpr (STEP) {
     __syncthreads();                             // every thread has read them
-    if (threadIdx.x == 0) { c.len[blockIdx.x] = len_step + n_step; c.next[blockIdx.x] = next_step + n_step; }
+    if (threadIdx.x == 0) {
+      c.len[blockIdx.x] = len_step + n_step;
+      c.next[blockIdx.x] = next_step + n_step;
+      if (t.taken != nullptr) t.taken[blockIdx.x] = n_step;
+    }
   }
 }
 
@@ -170,6 +174,7 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
   const int len = held_keys(c, r), next = c.next[r], n = t.count(c, r, len, next);
   c.len[r] = len + n;
   c.next[r] = next + n;
+  if (t.taken != nullptr) t.taken[r] = n;
 }
 
 // ---- attend ---------------------------------------------------------------------------------------------------------------------------

@@ -476,6 +476,7 @@ struct BoundedTokens {
   const void* q_norm_w; const void* k_norm_w; float eps;
   const float* cos_tab; const float* sin_tab; int max_pos;
   void* q_out;                             // [rows][L][Hq][D]
+  int32_t* taken;                          // [rows] or null: tokens that were taken (`counts` itself, it may be: written when nothing reads those any more)
   // tokens of row r that are taken: what is asked for, as far as there are slots and angles
   __device__ __forceinline__ int count(const BoundedCache& c, int r, int len, int next) const {
     const int n = counts != nullptr ? min(counts[r], L) : L;

@@ -395,7 +395,7 @@ int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_token
   if ((int64_t)b.rows * t->L > ((int64_t)1 << 31) / (t->Hq + 2 * b.Hkv) * 8) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_append: too many tokens for one call");
   MI_TRY(ready());
   return launch_bounded_append(b, BoundedTokens{t->qkv, t->ld_row, t->ld_token, t->L, t->Hq, t->counts, t->q_norm_w, t->k_norm_w, t->eps, t->cos_tab, t->sin_tab,
-                                                t->max_pos, t->q_out}, (hipStream_t)stream);
+                                                t->max_pos, t->q_out, t->taken}, (hipStream_t)stream);
 }
 
 uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq) {
