@@ -572,7 +572,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 // Bound by the matrix cores and the exponentials beside them, which hardly overlap: a block of 64 scores costs 16 cycles of the one and 15 to 20 of the other at D = 128.  4 prompts of 819 to 2048 bf16
 // tokens, 32 / 8 heads: 64 + 71 + 5 us, 2 x 37 GFLOP, 560 TFLOP/s over both passes (a product of 8192 x 8192 x 8192: 1135; the clock under this load is 1.95 GHz).  2 prompts of 700 float32 tokens 58 + 5
 // + 57 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
-// Workspace: [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
+// Workspace, rho of the queries that ask (`asking` a row at most): [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
 // queries, [slice][row][KV head][ld] sums.
 struct WeighWs { float* stats; float* parts; float* sums; int ld; };
 
@@ -829,7 +829,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 && !ALONE ? 3 : 2) vo
     }
     const int rho = rho0 + (wave * U + u) * 16 + ln;
     if (qd == 0 && rho < rhos) {
-      const size_t R = (size_t)a.L * G, rk = (size_t)r * c.Hkv + kh;
+      const size_t R = (size_t)a.asking() * G, rk = (size_t)r * c.Hkv + kh;
       if (splits == 1) {
         ws.stats[(rk * R + rho) * 2] = l[u] != 0.f ? m[u] : 0.f;
         ws.stats[(rk * R + rho) * 2 + 1] = l[u] != 0.f ? 1.f / l[u] : 0.f;
@@ -847,7 +847,7 @@ __global__ __launch_bounds__(256) void weigh_merge_kernel(BoundedCache c, Bounde
   const WeighRow w = weigh_row(c, a, r);
   const int rho = blockIdx.x * 256 + threadIdx.x;
   if (rho >= w.queries * G) return;
-  const size_t R = (size_t)a.L * G, rk = blockIdx.y;
+  const size_t R = (size_t)a.asking() * G, rk = blockIdx.y;
   const int have = max(1, (weigh_most(w, G, rho / queries * queries, queries) + chunk - 1) / chunk);       // slices with keys that the query's workgroups saw
   const float sc = a.scale * LOG2E;
   float M = LOWEST, L = 0.f;
@@ -905,7 +905,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && E <= 8 ? 3 : 2) void weigh_a
   }
   const float sc = a.scale * LOG2E;
   const size_t rk = (size_t)r * c.Hkv + kh;
-  const float* st_row = ws.stats + rk * a.L * G * 2;
+  const float* st_row = ws.stats + rk * a.asking() * G * 2;
   const T* q_row = (const T*)a.q + (((size_t)r * a.L + w.first) * a.Hq + kh * G) * D;
   const int64_t ld_q = (int64_t)a.Hq * D;
   float x[KS][4];
@@ -1292,7 +1292,7 @@ int attend_splits(const BoundedCache& c, int Hq, int ncu) {
 // 256 rows and heads of 1000 keys 53 / 58; 200 of 300 keys, 3 queries, 18 / 52.
 bool weigh_alone(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   const bool f32 = c.dtype == MI_F32;
-  const int64_t L = a.last > 0 ? std::min(a.last, a.L) : a.L;
+  const int64_t L = a.asking();
   if (L * (a.Hq / c.Hkv) > (f32 ? weigh_queries<float>() : weigh_queries<bf16>())) return false;
   return c.cap <= (f32 ? 128 : 288) || 4 * c.rows * c.Hkv >= 3 * ncu;
 }
@@ -1302,7 +1302,7 @@ bool weigh_alone(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
 struct WeighPlan { int splits, chunk, ks, per, slices; };
 WeighPlan weigh_plan(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   WeighPlan p;
-  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L, f32 = c.dtype == MI_F32, U = f32 ? 1 : 2;
+  const int G = a.Hq / c.Hkv, L = a.asking(), f32 = c.dtype == MI_F32, U = f32 ? 1 : 2;
   const int64_t pairs = (int64_t)c.rows * c.Hkv, groups = pairs * (((int64_t)L * G + 64 * U - 1) / (64 * U));
   const int64_t fit = std::max<int64_t>({(int64_t)c.cap * groups / ((f32 ? 16 : 8) * ncu), 256, (c.cap + MAX_SPLITS - 1) / MAX_SPLITS});
   p.chunk = (int)std::min<int64_t>((fit + 63) / 64 * 64, (c.cap + 63) / 64 * 64);
@@ -1332,7 +1332,7 @@ size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
 size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
   if (weigh_alone(c, a, ncu)) return 0;
   const WeighPlan p = weigh_plan(c, a, ncu);
-  const size_t one = up256((size_t)c.rows * a.Hq * a.L * 8), ld = ((size_t)c.cap + 3) & ~(size_t)3;
+  const size_t one = up256((size_t)c.rows * a.Hq * a.asking() * 8), ld = ((size_t)c.cap + 3) & ~(size_t)3;
   return one + std::max(p.splits > 1 ? one * p.splits : 0, p.slices > 1 ? (size_t)p.slices * c.rows * c.Hkv * ld * 4 : 0);
 }
 size_t bounded_evict_ws(const BoundedCache& c, int budget) {
@@ -1384,8 +1384,8 @@ int launch_bounded_attend(const BoundedCache& c, const BoundedAttend& a, void* w
 
 int launch_bounded_weigh(const BoundedCache& c, const BoundedWeigh& a, void* ws, int ncu, hipStream_t st) {
   const WeighPlan p = weigh_plan(c, a, ncu);
-  const int G = a.Hq / c.Hkv, L = a.last > 0 ? std::min(a.last, a.L) : a.L;
-  float* more = (float*)((char*)ws + up256((size_t)c.rows * a.Hq * a.L * 8));
+  const int G = a.Hq / c.Hkv, L = a.asking();
+  float* more = (float*)((char*)ws + up256((size_t)c.rows * a.Hq * L * 8));
   const WeighWs w{(float*)ws, more, more, (c.cap + 3) & ~3};
   const unsigned rhos = (unsigned)L * G, pairs = c.rows * c.Hkv;
   return by_type(c.dtype, [&](auto z) {

@@ -488,6 +488,7 @@ struct BoundedAttend {
 };
 struct BoundedWeigh {
   const void* q; int L, Hq, last; const int32_t* counts; float scale;         // q [rows][L][Hq][D]
+  __host__ __device__ int asking() const { return last > 0 && last < L ? last : L; }        // queries of a row, at most
 };
 bool bounded_head_dim(int D);
 bool bounded_group(int G);               // query heads per KV head
