@@ -37,6 +37,13 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _whole(*numbers) -> None:
+    # (ctypes cuts off what does not fit)
+    for n in numbers:
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise ValueError(f"{n}: a number of 32 bits")
+
+
 class BoundedKVCache:
     """``keys`` / ``values`` [rows, kv_heads, capacity, head_dim], or -- with ``block_table`` [rows, blocks a row] int32 -- arenas
     [blocks, kv_heads, block_tokens, head_dim] as the engine's paged caches have them (block_tokens a power of two from 16 on; a block
@@ -120,8 +127,9 @@ class BoundedKVCache:
                 self._check(t, "norm weights", self.dtype)
                 if t.shape != (D,) or not t.is_contiguous():
                     raise ValueError(f"norm weights: [{D}]")
+        _whole(tokens)
         q = qkv.new_empty((rows, tokens, heads, D))
-        a = L.OpBoundedTokens(qkv.data_ptr(), qkv.stride(0), qkv.stride(1), tokens, heads, self._counts(counts), _ptr(q_norm), _ptr(k_norm), eps, cos.shape[0],
+        a = L.OpBoundedTokens(qkv.data_ptr(), qkv.stride(0), qkv.stride(1), tokens, heads, self._counts(counts), _ptr(q_norm), _ptr(k_norm), eps, min(cos.shape[0], 2 ** 31 - 1),
                               cos.data_ptr(), sin.data_ptr(), q.data_ptr(), self.taken.data_ptr())
         self._call(self._lib.mi_op_bounded_append, self._ref, C.byref(a))
         return q
@@ -148,6 +156,7 @@ class BoundedKVCache:
         self._check(q, "q", self.dtype)
         if q.dim() != 4 or q.shape[0] != self.rows or q.shape[3] != self.head_dim:
             raise ValueError(f"q: [{self.rows}, tokens, heads, {self.head_dim}]")
+        _whole(last, q.shape[1])
         q = q.contiguous()
         n = self._lib.mi_op_bounded_weigh_ws(self._ref, q.shape[1], q.shape[2], last)
         ws = self._workspace(n)
@@ -157,6 +166,7 @@ class BoundedKVCache:
         """At most ``budget`` keys stay per row and KV head: those at the first ``keep_first`` positions and the last ``keep_last`` before all
         others, then the most weighted (NaN least), equal ones by the lower slot.  Kept keys behind slot `budget` move into the holes in front of it.
         Slots in blocks that the table does not name have no key: in front of `budget` they stay as they are and count in it, behind it they leave."""
+        _whole(budget, keep_first, keep_last)
         n = self._lib.mi_op_bounded_evict_ws(self._ref, budget)
         ws = self._workspace(n)
         self._call(self._lib.mi_op_bounded_evict, self._ref, budget, keep_first, keep_last, _ptr(ws), n)

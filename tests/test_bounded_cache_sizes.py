@@ -2,9 +2,11 @@
 from __future__ import annotations
 
 import pytest
+import torch
 
 from mlx_parallm_amd import _lib as L
-from tests.test_bounded_cache import P, PAGED, cache, refused, tokens
+from mlx_parallm_amd.bounded_cache import BoundedKVCache
+from tests.test_bounded_cache import P, PAGED, cache, parts, refused, tokens
 
 
 @pytest.mark.parametrize("rows", [1, 8])
@@ -19,3 +21,19 @@ def test_the_workspace_of_the_last_queries_does_not_grow_with_the_prompt(rows):
         assert one <= got <= one * 65 + 64 * rows * 8 * tokens_ * 4 + 1024
     c = cache(rows=rows, Hkv=8, D=128, cap=8001)
     assert lib.mi_op_bounded_weigh_ws(c, 8001, 40, 0) == lib.mi_op_bounded_weigh_ws(c, 8001, 40, 8001) >= rows * 40 * 8001 * 8
+
+
+@pytest.mark.parametrize("call", [
+    lambda c, n: c.evict(n), lambda c, n: c.evict(10, keep_first=n), lambda c, n: c.evict(10, keep_last=n),
+    lambda c, n: c.weigh(torch.zeros((2, 3, 4, 64), dtype=torch.bfloat16), last=n)])
+@pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 5, 2 ** 64 + 1, -2 ** 31 - 1, -2 ** 32 + 5])
+def test_numbers_of_more_than_32_bits_are_refused(call, n):
+    """(The binding would cut them off: a budget of 2^32 + 5 would leave five keys, keep_last = 2^32 protect none.)"""
+    with pytest.raises(ValueError, match="32 bits"):
+        call(BoundedKVCache(**parts()), n)
+
+
+def test_more_tokens_than_32_bits_count_are_refused():
+    qkv = torch.zeros((2, 1, 8 * 64), dtype=torch.bfloat16).expand(2, 2 ** 32 + 1, 8 * 64)
+    with pytest.raises(ValueError, match="32 bits"):
+        BoundedKVCache(**parts()).append(qkv, 4, torch.zeros((10, 32)), torch.zeros((10, 32)))
