@@ -1324,6 +1324,22 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 bool bounded_head_dim(int D) { return D == 16 || D == 32 || D == 64 || D == 96 || D == 128 || D == 192 || D == 256; }
 bool bounded_group(int G) { return G >= 1 && G <= MAX_GROUP; }
 
+// (a launch takes fewer than 2^32 threads; one that fails would leave those behind it with what it has not written)
+static int append_lane_bits(int D) {
+  int bits = 0;
+  while ((16 << bits) < D) ++bits;
+  return bits;
+}
+bool bounded_append_fits(const BoundedCache& c, const BoundedTokens& t) {
+  return (int64_t)c.rows * t.L <= (((int64_t)1 << 32) - 256) / ((t.Hq + 2 * c.Hkv) << append_lane_bits(c.D));
+}
+bool bounded_weigh_fits(const BoundedCache& c, const BoundedWeigh& a, int ncu) {
+  if (weigh_alone(c, a, ncu)) return true;
+  const WeighPlan p = weigh_plan(c, a, ncu);
+  const int64_t Q = c.dtype == MI_F32 ? weigh_queries<float>() : weigh_queries<bf16>(), pairs = (int64_t)c.rows * c.Hkv, most = (1 << 24) - 1;
+  return ((int64_t)a.asking() * (a.Hq / c.Hkv) + Q - 1) / Q * p.splits <= most / pairs && ((int64_t)c.cap + 64 * p.ks - 1) / (64 * p.ks) * p.slices <= most / pairs;
+}
+
 size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu) {
   if (attend_alone(c, Hq)) return 0;
   const size_t splits = attend_splits(c, Hq, ncu), ld = ((size_t)c.cap + 31) & ~(size_t)31;
@@ -1343,8 +1359,7 @@ size_t bounded_evict_ws(const BoundedCache& c, int budget) {
 }
 
 int launch_bounded_append(const BoundedCache& c, const BoundedTokens& t, hipStream_t st) {
-  int bits = 0;
-  while ((16 << bits) < c.D) ++bits;
+  const int bits = append_lane_bits(c.D);
   return by_type(c.dtype, [&](auto z) {
     using T = decltype(z);
     if ((int64_t)t.L * (t.Hq + 2 * c.Hkv) << bits <= STEP_TASKS) {

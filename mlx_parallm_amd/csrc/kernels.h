@@ -492,6 +492,8 @@ struct BoundedWeigh {
 };
 bool bounded_head_dim(int D);
 bool bounded_group(int G);               // query heads per KV head
+bool bounded_append_fits(const BoundedCache& c, const BoundedTokens& t);                  // one launch's threads
+bool bounded_weigh_fits(const BoundedCache& c, const BoundedWeigh& a, int ncu);
 size_t bounded_attend_ws(const BoundedCache& c, int Hq, int ncu);
 size_t bounded_weigh_ws(const BoundedCache& c, const BoundedWeigh& a, int ncu);
 size_t bounded_evict_ws(const BoundedCache& c, int budget);

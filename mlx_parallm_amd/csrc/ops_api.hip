@@ -392,10 +392,10 @@ int mi_op_bounded_append(const mi_op_bounded_cache* c, const mi_op_bounded_token
   const uint64_t es = dtype_size(b.dtype);
   if (((uintptr_t)t->qkv | (uintptr_t)t->q_out | (uintptr_t)t->q_norm_w | (uintptr_t)t->k_norm_w | (uint64_t)t->ld_row * es | (uint64_t)t->ld_token * es) % 16 != 0)
     return fail(MI_ERR_INVALID, "mi_op_bounded_append: arrays and strides are whole 16 bytes");
-  if ((int64_t)b.rows * t->L > ((int64_t)1 << 31) / (t->Hq + 2 * b.Hkv) * 8) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_append: too many tokens for one call");
+  const BoundedTokens n{t->qkv, t->ld_row, t->ld_token, t->L, t->Hq, t->counts, t->q_norm_w, t->k_norm_w, t->eps, t->cos_tab, t->sin_tab, t->max_pos, t->q_out, t->taken};
+  if (!bounded_append_fits(b, n)) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_append: too many tokens for one call");
   MI_TRY(ready());
-  return launch_bounded_append(b, BoundedTokens{t->qkv, t->ld_row, t->ld_token, t->L, t->Hq, t->counts, t->q_norm_w, t->k_norm_w, t->eps, t->cos_tab, t->sin_tab,
-                                                t->max_pos, t->q_out, t->taken}, (hipStream_t)stream);
+  return launch_bounded_append(b, n, (hipStream_t)stream);
 }
 
 uint64_t mi_op_bounded_attend_ws(const mi_op_bounded_cache* c, int Hq) {
@@ -429,8 +429,9 @@ int mi_op_bounded_weigh(const mi_op_bounded_cache* c, const void* q, int L, int 
   if ((int64_t)b.rows * L > ((int64_t)1 << 31) / Hq) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_weigh: too many tokens for one call");
   if (!q || (uintptr_t)q % 16 != 0) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: queries (aligned to 16 bytes)");
   if (!bounded_scale(scale)) return fail(MI_ERR_INVALID, "mi_op_bounded_weigh: the scale is positive and finite");
-  MI_TRY(ready());
   const BoundedWeigh a{q, L, Hq, last, counts, scale};
+  if (!bounded_weigh_fits(b, a, gemv_cu_count())) return fail(MI_ERR_UNSUPPORTED, "mi_op_bounded_weigh: too many tokens or slots for one call");
+  MI_TRY(ready());
   MI_TRY(bounded_workspace(ws, ws_bytes, bounded_weigh_ws(b, a, gemv_cu_count())));
   return launch_bounded_weigh(b, a, ws, gemv_cu_count(), (hipStream_t)stream);
 }

@@ -37,3 +37,14 @@ def test_more_tokens_than_32_bits_count_are_refused():
     qkv = torch.zeros((2, 1, 8 * 64), dtype=torch.bfloat16).expand(2, 2 ** 32 + 1, 8 * 64)
     with pytest.raises(ValueError, match="32 bits"):
         BoundedKVCache(**parts()).append(qkv, 4, torch.zeros((10, 32)), torch.zeros((10, 32)))
+
+
+def test_calls_of_more_threads_than_a_launch_takes_are_refused():
+    """2^32 threads in a launch: the first launch of such a call would fail, and those behind it would go on with what it has not written."""
+    lib = L.lib()
+    at = 2 ** 32 // (8 << 2) // 2                         # tokens of 8 heads of 64, four lanes each, in two rows
+    refused(lib.mi_op_bounded_append(cache(), tokens(L=at), None), -3, "too many")
+    refused(lib.mi_op_bounded_weigh(cache(rows=1, Hkv=1, D=16, dtype=L.MI_F32), P, 2 ** 31 - 1, 1, None, 0, 0.1, P, 1 << 62, None), -3, "too many")
+    refused(lib.mi_op_bounded_weigh(cache(rows=2000, Hkv=8, cap=1 << 20), P, 300, 8, None, 0, 0.1, P, 1 << 62, None), -3, "too many")
+    for rc in (lib.mi_op_bounded_append(cache(), tokens(L=0), None), lib.mi_op_bounded_weigh(cache(), P, 0, 4, None, 0, 0.1, P, 1 << 40, None)):
+        assert rc == -1
