@@ -70,7 +70,7 @@ int bounded_workspace(const void* ws, uint64_t have, uint64_t need) {
   return MI_OK;
 }
 
-bool bounded_scale(float s) { return s > 0.f && s < INFINITY; }
+bool bounded_scale(float s) { return s > 0.f && s * 1.4427f < INFINITY; }       // (exponents are to base 2)
 
 AttnShape to_shape(const mi_op_attn_shape* s) {
   return AttnShape{s->B, s->L, s->Hq, s->Hkv, s->D, s->act, s->kv, s->rnd, s->cap};

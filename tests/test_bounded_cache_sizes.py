@@ -48,3 +48,10 @@ def test_calls_of_more_threads_than_a_launch_takes_are_refused():
     refused(lib.mi_op_bounded_weigh(cache(rows=2000, Hkv=8, cap=1 << 20), P, 300, 8, None, 0, 0.1, P, 1 << 62, None), -3, "too many")
     for rc in (lib.mi_op_bounded_append(cache(), tokens(L=0), None), lib.mi_op_bounded_weigh(cache(), P, 0, 4, None, 0, 0.1, P, 1 << 40, None)):
         assert rc == -1
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_scales_that_are_infinite_to_base_2_are_refused(scale):
+    lib = L.lib()
+    refused(lib.mi_op_bounded_attend(cache(), P, 4, None, scale, P, P, 1 << 40, None), -1, "scale")
+    refused(lib.mi_op_bounded_weigh(cache(), P, 3, 4, None, 0, scale, P, 1 << 40, None), -1, "scale")
