@@ -188,11 +188,11 @@ __global__ void advance_kernel(BoundedCache c, BoundedTokens t) {
 // largest is 2^11 below is raised until it is not, the sums with it: by a power of two, which rounds nothing, and down again behind it.  A weight is off by 2^-27 of the largest of its tile of 32 keys at most.
 // What a key weighs needs the final maximum and sum of every head, so the products are kept (4 bytes a head and key, 3 % of 16-bit keys and values at 4 heads) and read by whoever has
 // them: the workgroup itself where it is alone (`ALONE`), else the joining launch.  (Adding them from here, relative to the slice's maximum, would have needed the same second pass.)
-// Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.4 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.6 us, of which 4 + 5 are the
-// launches' heads; 8 rows of 1025 float32 keys, 68 MB, 19.4 + 4.2: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
+// Bound by memory, once it runs: 4 x 32761 float16 keys, 32 / 8 heads of 128, 545 MB in 107 us (5.1 TB/s) + 9.6 to join; 32 rows of 0 to 2048 bf16 keys, 137 MB, 34 + 7.7 us, of which 4 + 5 are the
+// launches' heads; 8 rows of 1025 float32 keys, 68 MB, 19.3 + 4.2: four of the 16 columns of a float32 product are heads, 4 us of matrix work that nothing hides in so short a call.
 
 // P is 2^UP where the score is the largest, in the sums of weights and values alike.  Below one where values reach to the end of float32, whose sums then stay inside it: 2^16 of them at 2^8, the most that P
-// goes beyond it.
+// goes beyond it.  (Values below 2^-102 lose bits for that.)
 template <typename T>
 constexpr float UP = std::is_same_v<T, f16> ? 13.f : -24.f;
 
@@ -570,8 +570,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(BoundedCache c, Bounde
 // end), then the sum over the queries for every key.  The first keeps queries in registers and passes keys through LDS, the second the
 // other way round.
 // Bound by the matrix cores and the exponentials beside them, which hardly overlap: a block of 64 scores costs 16 cycles of the one and 15 to 20 of the other at D = 128.  4 prompts of 819 to 2048 bf16
-// tokens, 32 / 8 heads: 64 + 71 + 5 us, 2 x 37 GFLOP, 560 TFLOP/s over both passes (a product of 8192 x 8192 x 8192: 1135; the clock under this load is 1.95 GHz).  2 prompts of 700 float32 tokens 58 + 5
-// + 57 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
+// tokens, 32 / 8 heads: 64 + 72 + 5 us, 2 x 37 GFLOP, 560 TFLOP/s over both passes (a product of 8192 x 8192 x 8192: 1135; the clock under this load is 1.95 GHz).  2 prompts of 700 float32 tokens 58 + 5
+// + 56 + 5 us, 70 TFLOP/s of 151.  The last 64 queries of 8001 paged keys 18 + 5 + 14 us, 10.5 GFLOP: units of four tiles each wait for their first keys.
 // Workspace, rho of the queries that ask (`asking` a row at most): [row][KV head][rho][2]; with split keys [row][KV head][slice][rho][2] in front of the merge, and in the same place, with split
 // queries, [slice][row][KV head][ld] sums.
 struct WeighWs { float* stats; float* parts; float* sums; int ld; };
@@ -1011,8 +1011,8 @@ __global__ __launch_bounds__(256) void weigh_sum_kernel(BoundedCache c, BoundedW
 // A workgroup per row and KV head finds the budget-th largest of its keys' ranks (32-bit numbers in the order of the weights, protected keys
 // above all): a histogram over the range that is left, 2048 bins, until a bin stays whole -- at most three, one or two where the weights differ.  A
 // second launch moves keys and values: with the moves known it spreads over the chip.
-// 64 rows and heads of 8192 keys down to 1024: 12.8 us (a chain of barriers on 64 CUs; the first histogram's range is wasted on the gap between zero and the least weight) + 15 us to move 59 MB (3.9 TB/s in rows of
-// 256 bytes); 256 of 1025 down to 1024, in one launch: 8.5.
+// 64 rows and heads of 8192 keys down to 1024: 12.5 us (a chain of barriers on 64 CUs; the first histogram's range is wasted on the gap between zero and the least weight) + 15.7 us to move 59 MB (3.8 TB/s in rows of
+// 256 bytes); 256 of 1025 down to 1024, in one launch: 8.4.
 struct EvictWs { int32_t* counts; int2* moves; uint32_t* ranks; int most; };      // [row][KV head]; [row][KV head][most] (from, to); [row][KV head][cap]
 
 // Where more keys are protected than the budget holds, they alone are ranked (`crowded`).  A slot in a block that is none has no key: in front of `budget` it stays as it is (no hole, as nothing can be
@@ -1271,7 +1271,7 @@ bool attend_alone(const BoundedCache& c, int Hq) {
   return c.cap <= 512 && c.cap * ((G + 15) / 16) <= 1024 && ((c.cap + 31) & ~31) * G <= ALONE_SCORES;
 }
 // Slices of a row's keys, of u times 128: so many workgroups that they fill two rounds of two a CU (rows are of unequal lengths; long caches, whose slices are, one round) and leave little of
-// the last round empty.  us, 1 / 2 / 3 units a slice: 32 rows of 520 float32 keys, 40 / 8 heads, 37.5 / 44.4 / 37.4; 8 of 2815 46.3 / 45.3 / 43.5; 8 of 1025 24.8 / 27.8 (21.4 without a slice for the last key); 4 of 32761 float16 keys in 16 /
+// the last round empty.  (Two a CU is what float32 heads of 128 hold; 16-bit heads of 128 hold three, smaller ones more, and their slices were chosen by the times below, not by a count of their own.)  us, 1 / 2 / 3 units a slice: 32 rows of 520 float32 keys, 40 / 8 heads, 37.5 / 44.4 / 37.4; 8 of 2815 46.3 / 45.3 / 43.5; 8 of 1025 24.8 / 27.8 (21.4 without a slice for the last key); 4 of 32761 float16 keys in 16 /
 // 32 / 64 slices 117 / 120 / 126; 32 of 0 to 2048 in 2 / 4 / 8 47.4 / 44.0 / 46.8.
 int attend_splits(const BoundedCache& c, int Hq, int ncu) {
   const int64_t tiles = (int64_t)c.rows * c.Hkv * ((Hq / c.Hkv + 15) / 16), units = std::max(1, (c.cap - 32 + 127) / 128), slots = 2 * ncu;

@@ -165,3 +165,12 @@ def test_values_of_the_types_size(n, dtype):
     q[..., 0] = 8.0
     want = attend_with_infinities(s, 4, q)
     assert np.isfinite(want).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("n", [40, 700])
+def test_values_that_are_next_to_nothing(n, dtype):
+    """2^-98 and less of it: their sums keep their bits."""
+    s = Setup(n, 2, 1, 64, n, [n, n], dtype)
+    s.cache.values.copy_((torch.randn((2, 1, n, 64), generator=s.g).double() * 2.0 ** -98).to(DT[dtype]))
+    attend_with_infinities(s, 4)
