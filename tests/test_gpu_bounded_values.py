@@ -69,6 +69,22 @@ def test_infinite_values_of_keys_that_weigh_little(n, first, dtype):
     assert (attend_with_infinities(s, 2, q)[0, :, 1] == -INF).all()
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n,top,low", [(20, 18, 1), (20, 1, 18), (60, 58, 1), (500, 3, 490), (1200, 1198, 1), (1200, 1, 1198), (1200, 300, 310)])
+def test_infinite_values_of_keys_whose_weight_32_bits_do_not_hold(n, top, low, dtype):
+    """200 nats below the largest score, in the same tile, wave and slice and in others."""
+    D = 64
+    s = Setup(n, 1, 1, D, n, [n], dtype)
+    k = torch.zeros(n, D)
+    k[:, 0], k[top, 0], k[low, 0] = torch.rand(n, generator=s.g), 100.0, -100.0
+    s.cache.keys[0, 0] = k.to(DT[dtype]).cuda()
+    s.cache.values[0, 0, low, 1], s.cache.values[0, 0, low, 2] = -INF, INF
+    q = torch.zeros(1, 2, D, dtype=DT[dtype])
+    q[..., 0] = 8.0
+    want = attend_with_infinities(s, 2, q)
+    assert (want[0, :, 1] == -INF).all() and (want[0, :, 2] == INF).all()
+
+
 # ---- float16: weights far below the largest
 
 def exact(q, k, v):
